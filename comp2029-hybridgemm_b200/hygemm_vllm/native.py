@@ -13,6 +13,7 @@ from), and both precision partitions run in ONE persistent tcgen05 launch.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import importlib.machinery
 import importlib.util
@@ -108,6 +109,12 @@ def library():
     clip = [vp, vp, vp, vp, ci, ci, C.POINTER(ci), ci, ci]
     lib.hg_clip_pack.argtypes = clip + [vp]
     lib.hg_clip_pack_stats.argtypes = clip + [C.POINTER(C.c_double), vp]
+    lib.hg_norm.argtypes = [vp, ci, vp]
+    lib.hg_cache_page_bytes.argtypes, lib.hg_cache_page_bytes.restype = [ci, ci], C.c_int64
+    lib.hg_cache_write.argtypes = [vp, vp, vp, C.POINTER(C.c_int64), vp, ci, ci, vp]
+    lib.hg_cache_read.argtypes = [vp, vp, vp, vp, ci, ci, vp]
+    lib.hg_attention_workspace.argtypes, lib.hg_attention_workspace.restype = [vp, ci, ci, ci, ci], C.c_int64
+    lib.hg_attention.argtypes = [vp, vp, ci, vp]
     lib.hg_fused_error.restype = C.c_char_p
     lib.hg_fused_create.argtypes = [ci, pp, pp, vp, C.POINTER(vp)]
     lib.hg_fused_create_dtype.argtypes = [ci, pp, pp, vp, ci, C.POINTER(vp)]
@@ -142,6 +149,20 @@ def quantises_in_gemm(tokens: int, outputs: int) -> bool:
 
 def _stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+@contextlib.contextmanager
+def _switched(device):
+    with torch.cuda.device(device):
+        yield
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on_device(device):
+    """A context in which `device` is the current one (kernels are launched on the current device)."""
+    return _HERE if torch._C._cuda_getDevice() == device.index else _switched(device)
 
 
 def pack(x: torch.Tensor, fp4: bool = False):

@@ -8,11 +8,12 @@ Llama / Mistral MLPs through `linear_silu` for up to 128 tokens.
 """
 from __future__ import annotations
 
+import ctypes as C
 import os
 
 import torch
 
-from .native import DTYPES, _stream, library, scale_size
+from .native import DTYPES, _on_device, _stream, check, library, scale_size
 from .ops import _runtimes, linear_silu  # noqa: F401  (re-exported, reference layout)
 
 MAX_FUSED_TOKENS = 128
@@ -39,6 +40,90 @@ def silu_pack(x: torch.Tensor, math: int = 0, debug: bool = False):
         if status:
             raise RuntimeError(f"SwiGLU MX producer CUDA status {status}")
     return (q, sf, dbg) if debug else (q, sf)
+
+
+class NormCall(C.Structure):
+    """`hg_norm_call` of include/hygemm.h."""
+    _fields_ = [(name, C.c_void_p) for name in ("x", "residual", "gate", "post_weight", "weight", "stream_out", "normed", "codes", "scales")] + [
+        ("x_stride", C.c_int64), ("residual_stride", C.c_int64), ("gate_stride", C.c_int64), ("rows", C.c_int), ("k", C.c_int),
+        ("gate_per_row", C.c_int), ("eps", C.c_float), ("post_eps", C.c_float), ("scale", C.c_float)]
+
+
+def _rows_of(name, t, x):
+    """Checks a 16-bit matrix like `x` whose rows may be strided."""
+    if not (t.device == x.device and t.dtype == x.dtype and t.shape == x.shape and t.stride(1) == 1
+            and (t.shape[0] <= 1 or t.stride(0) % 8 == 0) and t.data_ptr() % 16 == 0):
+        raise ValueError(f"norm requires {name} [rows,K] of one 16-bit type and device, rows contiguous and aligned to 16 bytes")
+
+
+def _norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, packed):
+    if not (x.is_cuda and x.dtype in DTYPES and x.ndim == 2 and x.shape[1]):
+        raise ValueError("norm requires CUDA FP16/BF16 [rows,K]")
+    rows, k = x.shape
+    if k % (128 if packed else 8) or k > 32768:
+        raise ValueError("norm requires K divisible by 8, quantised by 128, and at most 32768")
+    _rows_of("x", x, x)
+    if residual is not None:
+        _rows_of("residual", residual, x)
+    for vector in (weight, post_weight):
+        if vector is not None and not (vector.device == x.device and vector.dtype == x.dtype and vector.shape == (k,)
+                                       and vector.is_contiguous() and vector.data_ptr() % 16 == 0):
+            raise ValueError("norm requires weights [K] of x's type and device, aligned to 16 bytes")
+    gate_stride = per_row = 0
+    if gate is not None:
+        if gate.device != x.device or gate.dtype != x.dtype or tuple(gate.shape) not in ((k,), (rows, k), (rows, 1)):
+            raise ValueError("norm requires a gate [K], [rows,K] or [rows,1] of x's type and device")
+        if gate.ndim == 2:
+            gate_stride = gate.stride(0)
+        per_row = int(gate.ndim == 2 and gate.shape[1] == 1 and k != 1)
+        if not per_row and (gate.stride(-1) != 1 or (rows > 1 and gate_stride % 8) or gate.data_ptr() % 16):
+            raise ValueError("norm requires a gate with contiguous rows aligned to 16 bytes")
+    if any(t is not None and t.requires_grad for t in (x, weight, residual, gate, post_weight)):
+        raise ValueError("norm has no gradient")
+    changed = residual is not None or gate is not None or post_weight is not None or scale != 1.0
+    stream = torch.empty((rows, k), dtype=x.dtype, device=x.device) if changed else x
+    normed = codes = sf = None
+    if packed:
+        codes = torch.empty((rows, k), dtype=torch.uint8, device=x.device)
+        sf = torch.empty(scale_size(rows, k), dtype=torch.uint8, device=x.device)
+    else:
+        normed = torch.empty((rows, k), dtype=x.dtype, device=x.device)
+    if rows:
+        pointers = (x, residual, gate, post_weight, weight, stream if changed else None, normed, codes, sf)
+        call = NormCall(*(None if t is None else t.data_ptr() for t in pointers), x.stride(0),
+                        residual.stride(0) if residual is not None else 0, gate_stride, rows, k, per_row, eps,
+                        eps if post_eps is None else post_eps, scale)
+        if rows == 1:   # the stride of a single row says nothing
+            call.x_stride = call.residual_stride = 0
+            call.gate_stride = 0
+        with _on_device(x.device):
+            check(library().hg_norm(C.byref(call), DTYPES[x.dtype], _stream(x.device)))
+    return (codes, sf, stream) if packed else (normed, stream)
+
+
+def norm_pack(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None, *,
+              gate: torch.Tensor | None = None, scale: float = 1.0, post_weight: torch.Tensor | None = None,
+              post_eps: float | None = None):
+    """Residual addition, RMS norm and MXFP8 quantisation in one kernel: `(q, sf, h)`.
+
+    `x` `[rows,K]` is a block's output in fp16 or bf16 (rows may be strided, as `residual`'s may), `h` the new residual stream and
+    `(q, sf)` the input of the next hybrid linear (`DualLinear.run_packed`):
+
+        y = x, or with `post_weight`  x / sqrt(mean(x^2) + post_eps) * post_weight
+        h = residual + scale * gate * y        rounded to x's type
+        n = h / sqrt(mean(h^2) + eps) * weight quantised as `native.pack` does, without a rounding to 16 bits before it
+
+    `gate` is `[K]`, `[rows,K]` or `[rows,1]`; `post_eps` defaults to `eps`.  Without residual, gate, scale and post norm `h` is
+    `x` itself.  K is a multiple of 128 up to 32768.  Forward only.
+    """
+    return _norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, True)
+
+
+def norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None, *,
+         gate: torch.Tensor | None = None, scale: float = 1.0, post_weight: torch.Tensor | None = None,
+         post_eps: float | None = None):
+    """`norm_pack` for a consumer in 16 bits (an unquantised lm_head, say): `(n, h)`.  K is a multiple of 8 up to 32768."""
+    return _norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, False)
 
 
 def _patch(mlp_class, method_types):

@@ -97,6 +97,73 @@ int hg_split_pack(const void* weight, int n_ids, int rows, int k, const int32_t*
 int hg_silu_pack(const void* in, void* q, void* sf, void* debug, int rows, int k, void* stream, int math);
 int hg_silu_pack_bf16(const void* in, void* q, void* sf, void* debug, int rows, int k, void* stream, int math);
 
+/* ---- What stands between the linears of a decoder block (no counterpart in the reference, which leaves it to the engine). ---- */
+
+/* Residual addition, RMS norm and MXFP8 quantisation of `rows` rows of `k` 16-bit values (HG_DTYPE_*):
+ *   y = x, or with a post weight x / sqrt(mean(x^2) + post_eps) * post_weight
+ *   h = round16(residual + scale * gate * y)     to stream_out [rows,k]
+ *   n = h / sqrt(mean(h^2) + eps) * weight       to codes [rows,k] and scales as hg_pack writes them, or to normed [rows,k] in 16 bits
+ * Sums are fp32; n is computed from the rounded h.  residual, gate and post_weight may be null.  gate[row * gate_stride + column], or
+ * with gate_per_row gate[row * gate_stride]; a stride of 0 is one row for all.  Strides count elements.  Without residual, gate,
+ * post_weight and with scale 1 h is x and stream_out is not written.  k is a multiple of 8 (codes: 128) up to 32768; pointers and rows are
+ * 16-byte aligned. */
+typedef struct hg_norm_call {
+  const void* x;
+  const void* residual;
+  const void* gate;
+  const void* post_weight;
+  const void* weight;
+  void* stream_out;
+  void* normed;                /* either this */
+  void* codes;                 /* or these two */
+  void* scales;
+  int64_t x_stride, residual_stride, gate_stride;
+  int rows, k, gate_per_row;
+  float eps, post_eps, scale;
+} hg_norm_call;
+int hg_norm(const hg_norm_call* call, int dtype, void* stream);
+
+/* A paged key-value cache in MXFP8: `pages` x kv_heads records of hg_cache_page_bytes, each page_size entries of one head:
+ * key codes [page_size][head_dim], value codes [page_size][head_dim], scale bytes [page_size][keys, values][head_dim / 32].
+ * A token's codes lie as [8][head_dim / 32][4], element d = 32 g + 4 x + i at (x, g, i).  head_dim is 64 or 128, page_size a
+ * multiple of 16 up to 1024, data 16-byte aligned. */
+typedef struct hg_cache {
+  void* data;
+  int pages, kv_heads, page_size, head_dim;
+} hg_cache;
+int64_t hg_cache_page_bytes(int page_size, int head_dim);
+/* Quantises k and v [tokens, kv_heads, head_dim] (16-bit; strides[4] = elements from token to token and from head to head of k, then of
+ * v, multiples of four) into the entries slots[token] = page * page_size + place.  A slot outside the cache is left out.  The
+ * slots of a call are distinct: what an entry named twice holds is not defined. */
+int hg_cache_write(const hg_cache* cache, const void* k, const void* v, const int64_t* strides, const int64_t* slots, int tokens,
+                   int dtype, void* stream);
+/* The entries slots[token] in 16 bits, k and v [tokens, kv_heads, head_dim]; zeros for a slot outside the cache. */
+int hg_cache_read(const hg_cache* cache, void* k, void* v, const int64_t* slots, int tokens, int dtype, void* stream);
+
+/* Attention of one new token a sequence over the cache.  Sequence i sees the positions p < length, and with a window only the
+ * last `window` of them; position p lies in page table[i * table_stride + p / page_size].  lengths[i] is taken as 0 when negative and as
+ * table_width * page_size when larger; positions of a page number outside the cache are left out.
+ *   out[i, h] = sum_p a_p v_p / sum_p a_p,  a_p = exp(scale q[i, h] . k_p)  over the head's kv head h / (heads / kv_heads)
+ * and zeros where nothing is seen.  q is [seqs, heads, head_dim] in 16 bits with q_stride elements from sequence to sequence (a
+ * multiple of eight).  Results go to out [seqs, heads, head_dim], or quantised as hg_pack writes [seqs, heads * head_dim] to codes
+ * and scales (heads * head_dim a multiple of 128); lse [seqs, heads] (optional) receives log(sum_p a_p), minus infinity where
+ * nothing is seen.  `workspace` has hg_attention_workspace bytes (16-byte aligned) and may be reused once the call has run. */
+typedef struct hg_attention_call {
+  const void* q;
+  const int* table;
+  const int* lengths;
+  void* out;                   /* either this */
+  void* codes;                 /* or these two */
+  void* scales;
+  float* lse;
+  void* workspace;
+  int64_t q_stride, table_stride;
+  int seqs, heads, table_width, window;   /* window 0: all positions */
+  float scale;
+} hg_attention_call;
+int64_t hg_attention_workspace(const hg_cache* cache, int seqs, int heads, int table_width, int window);
+int hg_attention(const hg_cache* cache, const hg_attention_call* call, int dtype, void* stream);
+
 /* integrations/vllm/native/runtime.cu:146-147 — build the schedule and workspace
  * for this exact shape (IEEE-half output).  A partition with rows==0 is skipped. */
 int hg_create(int low_id, int high_id, const hg_problem* low, const hg_problem* high, void* stream, void** handle);
