@@ -30,6 +30,7 @@
 #include <cstring>
 #include <mutex>
 #include <numeric>
+#include <type_traits>
 #include <vector>
 
 #include "hg_gemm_cluster.cuh"
@@ -72,6 +73,26 @@ struct ClusterParams {
   unsigned long long* trace;
 #endif
 };
+
+// Calls with an epilogue have instances of their own, with parameters behind the others': y = activation(sum + bias) + residual, all in
+// fp32 and rounded once.
+struct EpilogueParams : ClusterParams {
+  const uint16_t* bias;        // by output channel, or null
+  const uint16_t* residual;    // [tokens][outputs] with residual_stride elements from token to token, or null
+  int64_t residual_stride;
+  int activation;
+};
+template <bool EPILOGUE> using KernelParams = std::conditional_t<EPILOGUE, EpilogueParams, ClusterParams>;
+
+__device__ __forceinline__ float activated(float v, int activation) {
+  switch (activation) {
+    case HG_ACTIVATION_RELU: return v < 0.f ? 0.f : v;   // a NaN stays
+    case HG_ACTIVATION_SILU: return v / (1.f + expf(-v));
+    case HG_ACTIVATION_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678f));
+    case HG_ACTIVATION_GELU_TANH: return 0.5f * v * (1.f + tanhf(0.79788456f * (v + 0.044715f * v * v * v)));
+    default: return v;
+  }
+}
 
 // Partial tiles are exchanged in groups of four columns, [group][row][4] fp32; every slice owns a power of two of them.
 __host__ __device__ inline int share_log_of(int n_tile, int split) {
@@ -267,9 +288,9 @@ __host__ __device__ __forceinline__ int first_step(const ClusterParams& p, int s
 // WIDE: token tiles that start in the middle of a scale atom, a last tile wider than the others, units in turn (see ClusterPlan).  An
 // instance by itself: behind a quantiser, where its code is new to the instruction caches, a launch of it takes 0.3 us more (1536 x
 // 1536 at 887 tokens, quantiser included, 8.5 us against 8.8; behind another launch of its own both take 6.5).
-template <typename T, int PAIR, bool FUSED, bool WIDE>
+template <typename T, int PAIR, bool FUSED, bool WIDE, bool EPILOGUE = false>
 __global__ void __launch_bounds__(cluster_threads(PAIR, FUSED), 1)
-cluster_gemm_kernel(const __grid_constant__ ClusterParams p, const __grid_constant__ ClusterMaps maps) {
+cluster_gemm_kernel(const __grid_constant__ KernelParams<EPILOGUE> p, const __grid_constant__ ClusterMaps maps) {
   if (threadIdx.x == 0) HG_STAMP(0);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -588,6 +609,48 @@ cluster_gemm_kernel(const __grid_constant__ ClusterParams p, const __grid_consta
       const int channel = row_ok ? p.ids[w.part][row] : 0;   // fetched while the main loop runs
       const int valid = min(w.n, p.tokens - w.token0);
       char* const out_row = out + int64_t(channel) * (out_f32 ? 4 : 2) + int64_t(w.token0) * row_bytes;
+      // The epilogue's operands of this thread's row.  The residual of the columns that are stored next comes in while the ones before them are
+      // (the first ones' while the main loop runs): asked for where it is added, every sixteen columns waited for memory.
+      [[maybe_unused]] float bias = 0.f;
+      [[maybe_unused]] const uint16_t* residual_row = nullptr;
+      [[maybe_unused]] uint16_t residual[16] = {};
+      if constexpr (EPILOGUE) {
+        if (p.bias && row_ok) bias = to_float<T>(p.bias[channel]);
+        if (p.residual) residual_row = p.residual + channel + int64_t(w.token0) * p.residual_stride;
+      }
+      // Residual of N columns from column c on.
+      [[maybe_unused]] auto fetch_residual = [&](int c, auto columns) {
+        if constexpr (EPILOGUE) {
+          if (!residual_row || !row_ok) return;
+#pragma unroll
+          for (int i = 0; i < decltype(columns)::value; ++i)
+            if (c + i < valid) residual[i] = residual_row[int64_t(c + i) * p.residual_stride];
+        }
+      };
+      // In place, before the next columns' residual is fetched.
+      [[maybe_unused]] auto finish = [&](auto& v) {
+        if constexpr (EPILOGUE) {
+          constexpr int N = sizeof(v) / sizeof(float);
+          if (p.bias) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] += bias;
+          }
+          if (p.activation != HG_ACTIVATION_NONE) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = activated(v[i], p.activation);
+          }
+          if (residual_row) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] += to_float<T>(residual[i]);
+          }
+        }
+      };
+      using Four = std::integral_constant<int, 4>;
+      using Sixteen = std::integral_constant<int, 16>;
+      if constexpr (EPILOGUE) {
+        if (p.split > 1) fetch_residual(4 * ((slice << p.share_log) + side), Four{});
+        else if (active) fetch_residual(16 * (p.overlap && acc == 0 && 14 + side < ((w.n + 15) >> 4) ? 14 + side : side), Sixteen{});
+      }
       if (!warp_wait(acc_full_bar(acc), uint32_t(it >> 1) & 1u, abort_flag)) { error = kErrEpilogue; break; }
       tc_fence_after();
       if (threadIdx.x == 64 && it < 3) HG_STAMP(8 + 2 * it);
@@ -669,6 +732,10 @@ cluster_gemm_kernel(const __grid_constant__ ClusterParams p, const __grid_consta
 #pragma unroll
               for (int i = 0; i < 4; ++i) v[0][i] += v[s][i];
             }
+          if constexpr (EPILOGUE) {
+            finish(v[0]);
+            if (g + kSides < g_end) fetch_residual(4 * (g + kSides), Four{});
+          }
           store(4 * g, v[0]);
         }
       } else {
@@ -691,6 +758,10 @@ cluster_gemm_kernel(const __grid_constant__ ClusterParams p, const __grid_consta
           int next = begin > side && c == begin ? side : c + kSides;
           if (begin > side && next == begin) next = chunks;
           if (next < chunks) tc_load16(taddr + uint32_t(next) * 16u, a);
+          if constexpr (EPILOGUE) {
+            finish(r);
+            if (next < chunks) fetch_residual(16 * next, Sixteen{});
+          }
           store(16 * c, r);
           c = next;
         }
@@ -982,6 +1053,7 @@ ClusterPlan make_cluster_plan(int lo, int hi, int tokens, int k, const int max_c
 template <typename T, int PAIR, bool FUSED, bool WIDE = false>
 static void set_limits() {
   check(cudaFuncSetAttribute(cluster_gemm_kernel<T, PAIR, FUSED, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem), "cudaFuncSetAttribute");
+  check(cudaFuncSetAttribute(cluster_gemm_kernel<T, PAIR, FUSED, WIDE, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem), "cudaFuncSetAttribute");
 }
 
 void configure_cluster_kernels() {
@@ -1049,8 +1121,8 @@ ClusterPlan make_cluster_plan_for(int lo, int hi, int tokens, int k, int sms) {
   return make_cluster_plan(lo, hi, tokens, k, capacity_for(sms).data());
 }
 
-template <typename T, int PAIR, bool FUSED, bool WIDE = false>
-static cudaError_t launch(const ClusterPlan& plan, const ClusterParams& p, const ClusterMaps& maps, cudaStream_t stream, bool pdl) {
+template <typename T, int PAIR, bool FUSED, bool WIDE = false, bool EPILOGUE = false>
+static cudaError_t launch(const ClusterPlan& plan, const KernelParams<EPILOGUE>& p, const ClusterMaps& maps, cudaStream_t stream, bool pdl) {
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(unsigned(plan.clusters * plan.pair * plan.split));
   config.blockDim = dim3(FUSED ? first_act_warp(PAIR) * 32 + (p.tokens + 1) / 2 * 32 : cluster_threads(PAIR, false));
@@ -1068,7 +1140,7 @@ static cudaError_t launch(const ClusterPlan& plan, const ClusterParams& p, const
   }
   config.attrs = attribute;
   config.numAttrs = unsigned(count);
-  return cudaLaunchKernelEx(&config, cluster_gemm_kernel<T, PAIR, FUSED, WIDE>, p, maps);
+  return cudaLaunchKernelEx(&config, cluster_gemm_kernel<T, PAIR, FUSED, WIDE, EPILOGUE>, p, maps);
 }
 
 // What follows from the plan and the shape alone.
@@ -1139,7 +1211,14 @@ void launch_cluster(const ClusterPlan& plan, const ClusterCall& call, const Clus
 #endif
   const bool bf16 = call.dtype == HG_DTYPE_BF16;
   cudaError_t e;
-  if (call.x) e = bf16 ? launch<__nv_bfloat16, 1, true>(plan, p, maps, stream, pdl) : launch<__half, 1, true>(plan, p, maps, stream, pdl);
+  if (call.epilogue) {
+    const hg_epilogue& with = *call.epilogue;
+    EpilogueParams q{p, static_cast<const uint16_t*>(with.bias), static_cast<const uint16_t*>(with.residual), with.residual_stride, with.activation};
+    if (call.x) e = bf16 ? launch<__nv_bfloat16, 1, true, false, true>(plan, q, maps, stream, pdl) : launch<__half, 1, true, false, true>(plan, q, maps, stream, pdl);
+    else if (plan.pair == 1) e = bf16 ? launch<__nv_bfloat16, 1, false, false, true>(plan, q, maps, stream, pdl) : launch<__half, 1, false, false, true>(plan, q, maps, stream, pdl);
+    else if (plan.wide) e = bf16 ? launch<__nv_bfloat16, 2, false, true, true>(plan, q, maps, stream, pdl) : launch<__half, 2, false, true, true>(plan, q, maps, stream, pdl);
+    else e = bf16 ? launch<__nv_bfloat16, 2, false, false, true>(plan, q, maps, stream, pdl) : launch<__half, 2, false, false, true>(plan, q, maps, stream, pdl);
+  } else if (call.x) e = bf16 ? launch<__nv_bfloat16, 1, true>(plan, p, maps, stream, pdl) : launch<__half, 1, true>(plan, p, maps, stream, pdl);
   else if (plan.pair == 1) e = bf16 ? launch<__nv_bfloat16, 1, false>(plan, p, maps, stream, pdl) : launch<__half, 1, false>(plan, p, maps, stream, pdl);
   else if (plan.wide) e = bf16 ? launch<__nv_bfloat16, 2, false, true>(plan, p, maps, stream, pdl) : launch<__half, 2, false, true>(plan, p, maps, stream, pdl);
   else e = bf16 ? launch<__nv_bfloat16, 2, false>(plan, p, maps, stream, pdl) : launch<__half, 2, false>(plan, p, maps, stream, pdl);

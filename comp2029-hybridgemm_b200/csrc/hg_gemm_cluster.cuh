@@ -53,6 +53,7 @@ struct ClusterCall {
   int dtype;              // output type
   int* status;
   unsigned long long* trace;
+  const hg_epilogue* epilogue = nullptr;   // bias, activation and residual in the same launch, or null
 };
 // Boxes: weights 128 >> cut_log rows x 2 K128 blocks; activations n_step / pair and, for the last token tile, n_tail / pair rows;
 // scales (pairs only) 2 atoms.  Maps a launch does not use (an absent partition; activations quantised in the kernel) may

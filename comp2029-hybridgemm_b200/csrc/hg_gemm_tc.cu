@@ -1167,9 +1167,14 @@ static TcParams base_params(const Plan& plan, const hg_problem& l, const hg_prob
 }
 
 void tc_run(TcGemm* g, const hg_problem& l, const hg_problem& h, cudaStream_t stream, const void* x, int x_dtype,
-            const PartialTarget* partial) {
+            const PartialTarget* partial, const hg_epilogue* epilogue) {
   const bool fused = x != nullptr;
   validate(l, h, fused);
+  if (epilogue) {
+    if (!g->clustered || partial) throw std::runtime_error("An epilogue needs the automatic schedule");
+    if (epilogue->activation < HG_ACTIVATION_NONE || epilogue->activation > HG_ACTIVATION_GELU_TANH) throw std::runtime_error("Unknown activation");
+    if ((reinterpret_cast<uintptr_t>(epilogue->bias) | reinterpret_cast<uintptr_t>(epilogue->residual)) & 1) throw std::runtime_error("Bias and residual must be aligned");
+  }
   if (fused) {
     if ((g->clustered ? g->cluster.n_tile : g->plan.n_tile) != 16) throw std::runtime_error("Fused activation quantisation serves at most 16 tokens");
     if (x_dtype != HG_DTYPE_F16 && x_dtype != HG_DTYPE_BF16) throw std::runtime_error("Unknown activation dtype");
@@ -1224,6 +1229,7 @@ void tc_run(TcGemm* g, const hg_problem& l, const hg_problem& h, cudaStream_t st
 #ifdef HG_TRACE
     call.trace = g->d_trace;
 #endif
+    call.epilogue = epilogue;
     launch_cluster(g->cluster, call, hit->maps, stream, true);
     return;
   }

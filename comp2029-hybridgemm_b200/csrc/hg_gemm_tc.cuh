@@ -49,6 +49,7 @@ struct TcGemm;  // opaque device-side state (plan buffers, workspace, counters, 
 TcGemm* tc_create(const hg_problem& l, const hg_problem& h, int schedule, int dtype, cudaStream_t stream);
 // `x` (optional): 16-bit activations [tokens,k] to quantise inside the GEMM kernel (at most 16 tokens);
 // the problems' activation / activation_scales pointers are then ignored.
+// `epilogue` (optional, HG_SCHEDULE_AUTO only): bias, activation and residual of hg_linear_epilogue.
 // `partial` (optional): row-parallel tensor parallelism; the result goes to this rank's half of a peer-mapped
 // exchange buffer (see hg_run_partial) instead of the problems' `output`.
 struct PartialTarget {
@@ -58,7 +59,7 @@ struct PartialTarget {
   const int* state;    // device word counting finished exchanges
 };
 void tc_run(TcGemm*, const hg_problem& l, const hg_problem& h, cudaStream_t stream, const void* x = nullptr,
-            int x_dtype = HG_DTYPE_BF16, const PartialTarget* partial = nullptr);
+            int x_dtype = HG_DTYPE_BF16, const PartialTarget* partial = nullptr, const hg_epilogue* epilogue = nullptr);
 void tc_destroy(TcGemm*);
 // What the handle launches: the tile schedule (HG_SCHEDULE_AUTO: the cluster kernel), tokens per tile, K256 stages, shared memory,
 // the kernel's registers and local memory, and the activations' and scales' bytes of a stage.

@@ -45,6 +45,13 @@ struct Runner {
     return id >= HG_SCHEDULE_SIMT && id <= kLastSimtVariant;
   }
 
+  // With an epilogue in the tensor-core launch, whatever the launch policy: see hg_run_epilogue.
+  void run_epilogue(const hg_problem& l, const hg_problem& h, const void* x, int x_dtype, const hg_epilogue& epilogue, cudaStream_t s) {
+    if (!same_shape(l, low) || !same_shape(h, high)) throw std::runtime_error("Kernel cannot rebind to a different shape");
+    if (simt_only()) throw std::runtime_error("An epilogue needs the automatic schedule");
+    tc_run(tc, l, h, s, x, x_dtype, nullptr, &epilogue);
+  }
+
   void run(const hg_problem& l, const hg_problem& h, cudaStream_t s, int policy) {
     if (!same_shape(l, low) || !same_shape(h, high)) throw std::runtime_error("Kernel cannot rebind to a different shape");
     if (policy < 0 || policy > HG_POLICY_GEMV_PAIR4) throw std::runtime_error("Unknown launch policy");
@@ -111,7 +118,7 @@ int hg_run_x(void* handle, const hg_problem* l, const hg_problem* h, const void*
 
 // hg_linear and hg_linear_silu: quantise into the workspace and multiply, or (no workspace) both in one launch.
 static void run_linear(void* handle, const hg_problem* l, const hg_problem* h, const void* x, int x_dtype, bool swiglu, int math,
-                       void* workspace, void* output, cudaStream_t s) {
+                       void* workspace, void* output, cudaStream_t s, const hg_epilogue* epilogue = nullptr) {
   if (!handle || !l || !h || !x || !output || (swiglu && !workspace)) throw std::runtime_error("Null argument to a layer call");
   if (x_dtype != HG_DTYPE_F16 && x_dtype != HG_DTYPE_BF16) throw std::runtime_error("Unknown activation dtype");
   auto* runner = static_cast<hg::Runner*>(handle);
@@ -119,7 +126,8 @@ static void run_linear(void* handle, const hg_problem* l, const hg_problem* h, c
   low.output = high.output = output;
   if (!workspace) {
     low.activation = high.activation = low.activation_scales = high.activation_scales = nullptr;
-    runner->run_x(low, high, x, x_dtype, s);
+    if (epilogue) runner->run_epilogue(low, high, x, x_dtype, *epilogue, s);
+    else runner->run_x(low, high, x, x_dtype, s);
     return;
   }
   const int tokens = l->rows ? l->tokens : h->tokens, k = l->rows ? l->k : h->k;
@@ -129,7 +137,23 @@ static void run_linear(void* handle, const hg_problem* l, const hg_problem* h, c
   low.activation_scales = high.activation_scales = scales;
   if (swiglu) hg::silu_pack_activations(x, codes, scales, tokens, k, x_dtype, math, s);
   else hg::pack_activations(x, codes, scales, tokens, k, x_dtype, s);
-  runner->run(low, high, s, HG_POLICY_SERIAL);
+  if (epilogue) runner->run_epilogue(low, high, nullptr, x_dtype, *epilogue, s);
+  else runner->run(low, high, s, HG_POLICY_SERIAL);
+}
+
+int hg_run_epilogue(void* handle, const hg_problem* l, const hg_problem* h, const hg_epilogue* epilogue, void* stream) {
+  HG_TRY
+  if (!handle || !l || !h || !epilogue) throw std::runtime_error("Null argument to hg_run_epilogue");
+  static_cast<hg::Runner*>(handle)->run_epilogue(*l, *h, nullptr, HG_DTYPE_BF16, *epilogue, static_cast<cudaStream_t>(stream));
+  HG_CATCH
+}
+
+int hg_linear_epilogue(void* handle, const hg_problem* l, const hg_problem* h, const void* x, int x_dtype, void* workspace, void* output,
+                       const hg_epilogue* epilogue, void* stream) {
+  HG_TRY
+  if (!epilogue) throw std::runtime_error("Null argument to hg_linear_epilogue");
+  run_linear(handle, l, h, x, x_dtype, false, 0, workspace, output, static_cast<cudaStream_t>(stream), epilogue);
+  HG_CATCH
 }
 
 int hg_linear(void* handle, const hg_problem* l, const hg_problem* h, const void* x, int x_dtype, void* workspace, void* output, void* stream) {

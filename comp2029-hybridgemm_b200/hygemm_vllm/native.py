@@ -32,6 +32,11 @@ class Problem(C.Structure):
                 ("activation_scales", C.c_void_p), ("ids", C.c_void_p), ("output", C.c_void_p)]
 
 
+class Epilogue(C.Structure):
+    """`hg_epilogue` of include/hygemm.h."""
+    _fields_ = [("bias", C.c_void_p), ("residual", C.c_void_p), ("residual_stride", C.c_int64), ("activation", C.c_int)]
+
+
 PACK_MODE = int(os.environ.get("HYGEMM_PACK_MODE", "0"))
 # Calls of at most FUSED_QUANT_TOKENS tokens quantise the activations inside the GEMM kernel (`hg_run_x`: one launch instead of
 # two, identical bytes); HYGEMM_FUSED_QUANT=0 turns it off.
@@ -54,6 +59,8 @@ FUSED_QUANT_TOKENS_F32 = 16
 POLICIES = {"serial": 0, "concurrent": 1, "high_first": 2, "high_main": 3,
             "gemv_pair1": 4, "gemv_pair2": 5, "gemv_pair4": 6}
 DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+# Activations of an epilogue: max(x, 0), x / (1 + exp(-x)), x (1 + erf(x / sqrt 2)) / 2 and its approximation by tanh.
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 SPLIT_PACK_ROWS = 192512   # most rows hg_split_rows takes (its bitmap of the rows lives in shared memory)
 
@@ -109,6 +116,8 @@ def library():
     clip = [vp, vp, vp, vp, ci, ci, C.POINTER(ci), ci, ci]
     lib.hg_clip_pack.argtypes = clip + [vp]
     lib.hg_clip_pack_stats.argtypes = clip + [C.POINTER(C.c_double), vp]
+    lib.hg_run_epilogue.argtypes = [vp, pp, pp, C.POINTER(Epilogue), vp]
+    lib.hg_linear_epilogue.argtypes = [vp, pp, pp, vp, ci, vp, vp, C.POINTER(Epilogue), vp]
     lib.hg_norm.argtypes = [vp, ci, vp]
     lib.hg_cache_page_bytes.argtypes, lib.hg_cache_page_bytes.restype = [ci, ci], C.c_int64
     lib.hg_cache_write.argtypes = [vp, vp, vp, C.POINTER(C.c_int64), vp, ci, ci, vp]
@@ -273,6 +282,49 @@ class DualLinear:
         (28-34) and, of the launch policies, one of the four that enqueue it (the GEMV pairs and unknown ones are run_packed's)."""
         return not self.plans and not 28 <= self.low_id <= 34 and int(self.concurrent) in (0, 1, 2, 3)
 
+    def linear(self, x, bias=None, activation=None, residual=None):
+        """`activation(self(x) + bias) + residual` in the layer's own launch, added in fp32 and rounded once.
+
+        `bias` is `[outputs]`, `residual` `[tokens, outputs]` (rows may be strided), both of the layer's type; `activation` is one
+        of `ACTIVATIONS`.  Layers with the automatic schedule only.
+        """
+        if ACTIVATIONS.get(activation, -1) == 0 and bias is None and residual is None:
+            return self(x)
+        if x.ndim != 2 or x.shape[1] != self.k or x.device != self.w4.device or x.dtype not in DTYPES or not x.is_contiguous():
+            raise ValueError("HyGEMM input shape/device does not match its weights")
+        tokens = x.shape[0]
+        epilogue = self._epilogue(tokens, bias, activation, residual, x)
+        y = torch.empty((tokens, self.outputs), dtype=self.dtype, device=x.device)
+        if not tokens:
+            return y
+        # Fresh scratch per call: under CUDA-graph capture the graph's pool owns it.
+        scratch = (None if quantises_in_gemm(tokens, self.outputs) else
+                   torch.empty(tokens * self.k + scale_size(tokens, self.k), dtype=torch.uint8, device=x.device))
+        low, high = self.problems(x, x, y)
+        with _on_device(x.device):
+            stream = _stream(x.device)
+            handle = self._handle(tokens, 0, 0, C.byref(low), C.byref(high), stream)
+            check(library().hg_linear_epilogue(handle, C.byref(low), C.byref(high), x.data_ptr(), DTYPES[x.dtype],
+                                               None if scratch is None else scratch.data_ptr(), y.data_ptr(), C.byref(epilogue), stream))
+        self.calls[tokens] = self.calls.get(tokens, 0) + 1
+        return y
+
+    def _epilogue(self, tokens, bias, activation, residual, x):
+        """The checked operands of an epilogue, as the library takes them."""
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"HyGEMM epilogue activation must be one of {sorted(a for a in ACTIVATIONS if a)}")
+        if self.plans or self.low_id or self.high_id or not self._tensor_core():
+            raise ValueError("HyGEMM epilogue requires a layer with the automatic schedule")
+        if bias is not None and not (bias.device == x.device and bias.dtype == self.dtype and bias.shape == (self.outputs,) and bias.is_contiguous()):
+            raise ValueError("HyGEMM epilogue requires a contiguous bias [outputs] of the layer's type and device")
+        if residual is not None and not (residual.device == x.device and residual.dtype == self.dtype
+                                         and residual.shape == (tokens, self.outputs) and (residual.stride(1) == 1 or self.outputs == 1)):
+            raise ValueError("HyGEMM epilogue requires a residual [tokens, outputs] of the layer's type and device with contiguous rows")
+        if any(t is not None and t.requires_grad for t in (x, bias, residual)):
+            raise ValueError("HyGEMM layers have no gradient")
+        return Epilogue(None if bias is None else bias.data_ptr(), None if residual is None or not tokens else residual.data_ptr(),
+                        0 if residual is None else residual.stride(0), ACTIVATIONS[activation])
+
     def silu_linear(self, x, math):
         """This layer on SwiGLU of `x` = gate||up `[tokens, 2K]`: `producer.silu_pack` followed by `run_packed`."""
         native_path = _host is not None and math in (0, 1, 2)   # it takes a negative one for a call without SwiGLU
@@ -338,8 +390,8 @@ class DualLinear:
             prob.activation, prob.activation_scales, prob.output = qp, sp, yp
         return pair
 
-    def run_packed(self, q, sf):
-        """GEMM on already-quantised activations (reference: native.py:75-107)."""
+    def run_packed(self, q, sf, bias=None, activation=None, residual=None):
+        """GEMM on already-quantised activations (reference: native.py:75-107); bias, activation and residual as in `linear`."""
         if q.dtype != torch.uint8 or q.ndim != 2 or q.shape[1] != self.k or q.device != self.w4.device \
                 or not q.is_contiguous():
             raise ValueError("Invalid prepacked MXFP8 activation")
@@ -347,6 +399,9 @@ class DualLinear:
         if sf.dtype != torch.uint8 or sf.device != q.device or not sf.is_contiguous() \
                 or sf.numel() != scale_size(tokens, self.k):
             raise ValueError("Invalid prepacked MXFP8 scale buffer")
+        epilogue = None
+        if bias is not None or residual is not None or ACTIVATIONS.get(activation, -1):
+            epilogue = self._epilogue(tokens, bias, activation, residual, q)
         # Fresh output per call: under CUDA-graph capture the graph's pool owns it.
         y = torch.empty((tokens, self.outputs), dtype=self.dtype, device=q.device)
         if tokens == 0:
@@ -359,7 +414,11 @@ class DualLinear:
             low_id, high_id, policy = plan["low_id"], plan["high_id"], POLICIES[plan["policy"]]
             self.plans_used[tokens] = [plan["tokens"], low_id, high_id, policy]
         handle = self._handle(tokens, low_id, high_id, low_ref, high_ref, stream)
-        status = _lib.hg_run(handle, low_ref, high_ref, stream, policy)
+        if epilogue is None:
+            status = _lib.hg_run(handle, low_ref, high_ref, stream, policy)
+        else:
+            with _on_device(q.device):
+                status = _lib.hg_run_epilogue(handle, low_ref, high_ref, C.byref(epilogue), stream)
         if status:
             check(status)
         self.calls[tokens] = self.calls.get(tokens, 0) + 1

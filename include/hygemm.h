@@ -190,6 +190,21 @@ int hg_linear(void* handle, const hg_problem* low, const hg_problem* high, const
 /* The same for the SwiGLU of `x` = gate||up [tokens,2k]: hg_silu_pack (`math` as there) into the workspace, then hg_run. */
 int hg_linear_silu(void* handle, const hg_problem* low, const hg_problem* high, const void* x, int x_dtype, int math,
                    void* workspace, void* output, void* stream);
+/* What follows the product in the same launch (no counterpart in the reference): out = activation(sum + bias) + residual, in fp32
+ * and rounded once.  bias [outputs] and residual [tokens,outputs] (residual_stride elements from token to token) are of the
+ * output's type, either may be null; residual may be the output itself.  hg_run_epilogue is hg_run with it, hg_linear_epilogue
+ * hg_linear.  Handles of HG_SCHEDULE_AUTO only. */
+enum { HG_ACTIVATION_NONE = 0, HG_ACTIVATION_RELU = 1, HG_ACTIVATION_SILU = 2, HG_ACTIVATION_GELU = 3, /* x (1 + erf(x / sqrt 2)) / 2 */
+       HG_ACTIVATION_GELU_TANH = 4 };  /* x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 */
+typedef struct hg_epilogue {
+  const void* bias;
+  const void* residual;
+  int64_t residual_stride;
+  int activation;
+} hg_epilogue;
+int hg_run_epilogue(void* handle, const hg_problem* low, const hg_problem* high, const hg_epilogue* epilogue, void* stream);
+int hg_linear_epilogue(void* handle, const hg_problem* low, const hg_problem* high, const void* x, int x_dtype, void* workspace,
+                       void* output, const hg_epilogue* epilogue, void* stream);
 /* integrations/vllm/native/runtime.cu:151-161 — 10 ints per partition: id, tile_m,
  * tile_n, tile_k, stages, registers, shared bytes, local bytes, fp8, pingpong (-1 if absent).  They describe the kernel the
  * handle launches on prepacked activations; id 0 (HG_SCHEDULE_AUTO) is the cluster kernel, whose tile_m is the height of a
