@@ -19,6 +19,7 @@ import ctypes as C
 
 import torch
 
+from . import native
 from .native import DTYPES, _on_device, _stream, check, library, scale_size
 
 
@@ -56,9 +57,6 @@ class PagedCache:
             raise ValueError("PagedCache requires contiguous CUDA uint8 [pages, kv_heads, page_bytes(page_size, head_dim)]")
         self.data, self.page_size, self.head_dim = data, page_size, head_dim
         self.pages, self.kv_heads = data.shape[:2]
-        self._struct = Cache(data.data_ptr(), self.pages, self.kv_heads, page_size, head_dim)
-        self._ref = C.byref(self._struct)
-        self._workspaces = {}   # (sequences, heads, table width, window) -> bytes
 
     @classmethod
     def allocate(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, device="cuda"):
@@ -67,15 +65,20 @@ class PagedCache:
             raise ValueError("PagedCache requires pages and heads")
         return cls(torch.zeros((pages, kv_heads, page_bytes(page_size, head_dim)), dtype=torch.uint8, device=device), page_size, head_dim)
 
-    def _slots(self, slots, tokens=None):
-        if not (slots.device == self.data.device and slots.dtype == torch.int64 and slots.ndim == 1 and slots.is_contiguous()
-                and (tokens is None or slots.shape[0] == tokens)):
+    def _struct(self):
+        return C.byref(Cache(self.data.data_ptr(), self.pages, self.kv_heads, self.page_size, self.head_dim))
+
+    def _slots(self, slots):
+        if not (slots.device == self.data.device and slots.dtype == torch.int64 and slots.ndim == 1 and slots.is_contiguous()):
             raise ValueError("PagedCache requires contiguous int64 slots [tokens] on its device")
 
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Quantises `k` and `v` `[tokens, kv_heads, head_dim]` (fp16 or bf16; slices of a qkv output will do) into the entries
         `slots` (int64).  A slot outside the cache, such as the -1 of a padded batch, is left out.  The slots of a call are
         distinct: what an entry named twice holds afterwards is not defined."""
+        host = native._host
+        if host is not None and host.cache_write(self.data, self.page_size, self.head_dim, k, v, slots):
+            return
         shape = (slots.shape[0] if slots.ndim else -1, self.kv_heads, self.head_dim)
         for x in (k, v):
             if not (x.device == self.data.device and x.dtype in DTYPES and x.dtype == k.dtype and x.shape == shape):
@@ -89,11 +92,15 @@ class PagedCache:
             return
         strides = (C.c_int64 * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
         with _on_device(self.data.device):
-            check(library().hg_cache_write(self._ref, k.data_ptr(), v.data_ptr(), strides, slots.data_ptr(), shape[0],
+            check(library().hg_cache_write(self._struct(), k.data_ptr(), v.data_ptr(), strides, slots.data_ptr(), shape[0],
                                            DTYPES[k.dtype], _stream(self.data.device)))
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
         """The entries `slots` as `(k, v)`, each `[tokens, kv_heads, head_dim]` in `dtype`; zeros for a slot outside the cache."""
+        if native._host is not None and dtype in DTYPES:
+            got = native._host.cache_read(self.data, self.page_size, self.head_dim, slots, DTYPES[dtype])
+            if got is not None:
+                return got
         self._slots(slots)
         if dtype not in DTYPES:
             raise ValueError("PagedCache.read gives FP16 or BF16")
@@ -101,7 +108,7 @@ class PagedCache:
         k, v = (torch.empty((tokens, self.kv_heads, self.head_dim), dtype=dtype, device=self.data.device) for _ in (0, 1))
         if tokens:
             with _on_device(self.data.device):
-                check(library().hg_cache_read(self._ref, k.data_ptr(), v.data_ptr(), slots.data_ptr(), tokens, DTYPES[dtype],
+                check(library().hg_cache_read(self._struct(), k.data_ptr(), v.data_ptr(), slots.data_ptr(), tokens, DTYPES[dtype],
                                               _stream(self.data.device)))
         return k, v
 
@@ -128,6 +135,10 @@ class PagedCache:
         return self._attend(q, page_table, lengths, scale, window, lse, True)
 
     def _attend(self, q, page_table, lengths, scale, window, lse, packed):
+        if native._host is not None:
+            got = native._host.attention(self.data, self.page_size, self.head_dim, q, page_table, lengths, scale, window, lse, packed)
+            if got is not None:
+                return got
         device = self.data.device
         if not (q.device == device and q.dtype in DTYPES and q.ndim == 3 and q.shape[2] == self.head_dim and q.shape[1]
                 and q.shape[1] % self.kv_heads == 0):
@@ -156,13 +167,10 @@ class PagedCache:
         if lse:
             sums = torch.empty((rows, heads), dtype=torch.float32, device=device)
         if rows:
-            lib, key = library(), (rows, heads, width, window)
-            size = self._workspaces.get(key)
-            if size is None:
-                size = self._workspaces[key] = lib.hg_attention_workspace(self._ref, *key)
-                if size < 0:
-                    del self._workspaces[key]
-                    check(size)
+            lib, cache = library(), self._struct()
+            size = lib.hg_attention_workspace(cache, rows, heads, width, window)
+            if size < 0:
+                check(-1)
             # A fresh workspace per call: under CUDA-graph capture the graph's pool owns it.
             workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
             call = AttentionCall(q.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), out.data_ptr() if out is not None else None,
@@ -171,6 +179,6 @@ class PagedCache:
                                  page_table.stride(0), rows, heads, width, window,
                                  self.head_dim ** -0.5 if scale is None else scale)
             with _on_device(device):
-                check(lib.hg_attention(self._ref, C.byref(call), DTYPES[q.dtype], _stream(device)))
+                check(lib.hg_attention(cache, C.byref(call), DTYPES[q.dtype], _stream(device)))
         result = (codes, sf) if packed else (out,)
         return result + (sums,) if lse else result if packed else out

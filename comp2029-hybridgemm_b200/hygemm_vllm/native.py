@@ -134,7 +134,9 @@ def library():
     if _HOST_EXTENSION.exists():
         loader = importlib.machinery.ExtensionFileLoader("_hygemm_host", str(_HOST_EXTENSION))
         host = importlib.util.module_from_spec(importlib.util.spec_from_loader("_hygemm_host", loader))
-        host.bind(*(C.cast(f, vp).value for f in (lib.hg_linear, lib.hg_linear_silu, lib.hg_last_error)))
+        host.bind(*(C.cast(f, vp).value for f in (lib.hg_linear, lib.hg_linear_silu, lib.hg_last_error, lib.hg_linear_epilogue,
+                                                             lib.hg_norm, lib.hg_cache_write, lib.hg_cache_read, lib.hg_attention,
+                                                             lib.hg_attention_workspace)))
         _host = host
     _lib = lib
     return lib
@@ -288,12 +290,20 @@ class DualLinear:
         `bias` is `[outputs]`, `residual` `[tokens, outputs]` (rows may be strided), both of the layer's type; `activation` is one
         of `ACTIVATIONS`.  Layers with the automatic schedule only.
         """
-        if ACTIVATIONS.get(activation, -1) == 0 and bias is None and residual is None:
+        number = ACTIVATIONS.get(activation, -1)
+        if number == 0 and bias is None and residual is None:
             return self(x)
+        if number >= 0 and _host is not None and not PACK_MODE:
+            y = _host.forward_epilogue(self, x, bias, number, residual)
+            if y is not None:
+                return y
         if x.ndim != 2 or x.shape[1] != self.k or x.device != self.w4.device or x.dtype not in DTYPES or not x.is_contiguous():
             raise ValueError("HyGEMM input shape/device does not match its weights")
         tokens = x.shape[0]
         epilogue = self._epilogue(tokens, bias, activation, residual, x)
+        if tokens and _host is not None and not PACK_MODE and tokens not in self._ready and not x.requires_grad:
+            with _on_device(x.device):
+                self._prepare(x)   # the calls that follow go through the host extension
         y = torch.empty((tokens, self.outputs), dtype=self.dtype, device=x.device)
         if not tokens:
             return y
@@ -339,7 +349,15 @@ class DualLinear:
         return self._prepared(x, math)
 
     def _prepared(self, x, math):
-        """Prepares plain calls with this token count (handle, operand structs, workspace sizes; kept between calls) and makes one."""
+        """Prepares plain calls with this token count and makes one."""
+        self._prepare(x)
+        result = _host.forward(self, x, math)
+        if result is None:
+            raise RuntimeError("HyGEMM layer call was not prepared")
+        return result
+
+    def _prepare(self, x):
+        """What plain calls with this token count need: handle, operand structs, workspace sizes; kept between calls."""
         tokens = x.shape[0]
         y = torch.empty((tokens, self.outputs), dtype=self.dtype, device=x.device)
         low, high = self.problems(x, x, y)
@@ -349,10 +367,6 @@ class DualLinear:
             fused = (1 if tokens == 1 else 2) if fused and self.outputs <= FUSED_QUANT_MAX_OUTPUTS else 0
         self._ready[tokens] = _host.prepare(self, tokens, handle.value, C.addressof(low), C.addressof(high), (low, high), y,
                                             tokens * self.k + scale_size(tokens, self.k), fused)
-        result = _host.forward(self, x, math)
-        if result is None:
-            raise RuntimeError("HyGEMM layer call was not prepared")
-        return result
 
     def _handle(self, tokens, low_id, high_id, low_ref, high_ref, stream):
         """GEMM handle of one (token count, schedule ids) pair, created on first use: never during stream

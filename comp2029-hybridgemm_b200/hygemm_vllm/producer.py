@@ -13,6 +13,7 @@ import os
 
 import torch
 
+from . import native
 from .native import DTYPES, _on_device, _stream, check, library, scale_size
 from .ops import _runtimes, linear_silu  # noqa: F401  (re-exported, reference layout)
 
@@ -56,6 +57,8 @@ def _rows_of(name, t, x):
         raise ValueError(f"norm requires {name} [rows,K] of one 16-bit type and device, rows contiguous and aligned to 16 bytes")
 
 
+# What follows is called through the host extension where that takes a call (`native._host`); here is what it does otherwise, and what is
+# wrong with a call that neither takes.
 def _norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, packed):
     if not (x.is_cuda and x.dtype in DTYPES and x.ndim == 2 and x.shape[1]):
         raise ValueError("norm requires CUDA FP16/BF16 [rows,K]")
@@ -116,14 +119,18 @@ def norm_pack(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual
     `gate` is `[K]`, `[rows,K]` or `[rows,1]`; `post_eps` defaults to `eps`.  Without residual, gate, scale and post norm `h` is
     `x` itself.  K is a multiple of 128 up to 32768.  Forward only.
     """
-    return _norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, True)
+    host = native._host
+    got = None if host is None else host.norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, True)
+    return _norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, True) if got is None else got
 
 
 def norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None, *,
          gate: torch.Tensor | None = None, scale: float = 1.0, post_weight: torch.Tensor | None = None,
          post_eps: float | None = None):
     """`norm_pack` for a consumer in 16 bits (an unquantised lm_head, say): `(n, h)`.  K is a multiple of 8 up to 32768."""
-    return _norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, False)
+    host = native._host
+    got = None if host is None else host.norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, False)
+    return _norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, False) if got is None else got
 
 
 def _patch(mlp_class, method_types):

@@ -393,4 +393,4 @@ def test_refusals():
                            (data[:0], 16, 64), (data, 16, 96), (data, 0, 64), (data, 2048, 64)):
         with pytest.raises(ValueError):
             PagedCache(bad, page, dim)
-    assert native.library().hg_attention_workspace(cache._ref, 1, 3, 1, 0) == -1
+    assert native.library().hg_attention_workspace(cache._struct(), 1, 3, 1, 0) == -1
