@@ -2,22 +2,29 @@
 //
 //   s_t = scale q . k_t      p_t = exp(s_t - max s)      out = sum_t p_t v_t / sum_t p_t
 //
-// One pass over the cache with a running maximum and sum.  A unit of work is a run of 16-token tiles of one sequence, kv head and
-// up to eight of its query heads; a block of four warps takes one unit, its warps every fourth tile each, without shared memory on the
-// way: a tile's codes go from global memory straight into the fragments of two matrix products,
+// One pass over the cache with a running maximum and sum, in one launch.  A unit of work is a sequence, a kv head and up to eight of its
+// query heads.  A cluster of blocks takes one unit, each block a run of its 16-token tiles, each warp of a block every fourth of these;
+// the blocks' sums meet in shared memory.  A tile comes in by TMA, a few tiles ahead, into a ring that the warp has for itself, and
+// goes from there into the fragments of two matrix products,
 //   S^T [16 tokens, 8 heads]     = K [16 tokens, d]   Q^T [d, 8 heads]       (m16n8k16, one accumulator for every scale group of 32 d)
 //   O^T [16 d, 8 heads]          = V^T [16 d, tokens] P^T [tokens, 8 heads]
-// so that the heads fill the narrow side of an instruction, whatever their number, and the cache its wide one.  Codes become halves,
-// which hold them exactly.  Scales stay outside: those of the keys multiply a group's partial sum, those of the values the
-// probabilities, once for every group, before these are rounded to halves for the second product.
+// so that the heads fill the narrow side of an instruction, whatever their number, and the cache its wide one.  (tcgen05 would
+// take 128 rows where there are eight heads, and has no operand for scales along the summed axis of the second product; E4M3
+// operands of mma.sync are converted by instructions too here.)  Codes become halves, which hold them exactly.  Scales stay outside:
+// those of the keys multiply a group's partial sum, those of the values the probabilities, once for every group, before these are
+// rounded to halves.
 //
-// Roundings: q keeps its 16 bits (bf16 queries become halves under one power of two for the block, which keeps eight bits of
-// all that is not 2^-30 of the largest).  P times the scale is rounded to 11 bits (2^-12 of each weight), held between 2^-32 and
-// 2^8 of the largest so far by a bias of 2^7 and lazy rescaling.  Sums, maxima and outputs are fp32.
+// Roundings: q keeps its 16 bits (a head's bf16 queries become halves under a power of two, which keeps eight bits of all that is
+// not 2^-29 of the largest).  P times the scale of its values is rounded to 11 bits (2^-11 of each weight at most), held
+// between 2^-32 and 2^8 of the largest so far by a bias of 2^7 and lazy rescaling.  Sums, maxima and outputs are fp32.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
+#include <mutex>
+#include <type_traits>
 
 #include "hg_cache.cuh"
+#include "hg_gemm_cluster.cuh"
 
 namespace hg {
 namespace {
@@ -26,24 +33,36 @@ constexpr int kTile = 16;            // tokens of a step of one warp
 constexpr int kHeadTile = 8;         // query heads of a unit
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kBlocksPerSm = 3;
+constexpr int kRing = 3;             // tiles of a warp in shared memory or on their way there
 constexpr int kWhole = 16;           // sequences of no more tiles are not split
 constexpr int kUnitCost = 8;         // cost of a unit beside its tiles, in tiles
 constexpr int kLeastShare = 24;      // a block's share of the cost, where there is less for all blocks
+constexpr int kMostSplit = 16;       // blocks of a cluster at most
+constexpr int kFew = 8192;           // tiles of all units that are left to clusters
+constexpr int kMeet = 8;             // blocks whose sums are under way together
 constexpr float kBias = 7.f, kSlack = 4.f;   // P is kept in [0, 2^(kBias + 2 kSlack)]
 constexpr float kNone = -1e30f;      // maximum of nothing
+constexpr int kLeastScale = 24;      // values are summed under 2^-103 at least
 
-// The work of a split call is a line on which every unit (sequence and head unit, in this order) has its tiles behind kUnitCost
-// for what it costs besides; a block takes an equal share of the line, so whatever the lengths all blocks end together.
-// It holds parts of at most two units that other blocks have parts of, at its beginning and at its end.
-struct Join { int seq, head_unit, first, parts; };   // sums of a unit: slots first, 2 * (first / 2 + 1), + 2, ...
+// How units come to blocks.  Few units (CLUSTER): a cluster of `split` blocks each, whose sums meet in shared memory.  Many (LINE):
+// the work is a line on which every unit (sequence and head unit, in this order) has its tiles behind kUnitCost for what it costs
+// besides, and a block takes an equal share of it, so whatever the lengths all blocks end together.  A unit that ends in another
+// block than it begins in is added up by the one that it begins in, which comes to it last; the others come to their
+// parts of it first, write their sums to a slot and set a tag behind them, and the first one waits for the tags and takes them back.
+// It waits for blocks behind it alone, whose first parts wait for nothing, so the wait ends even where the device holds fewer blocks
+// than there are: all but one of them end.  A tag is 64 bits that a workspace holds by accident once in 2^64 slots, so it
+// needs no clearing, and no two calls share one.
+constexpr uint64_t kTag = 0x9d3f6ac1e57b2480ull;
 
 struct AttentionParams {
   hg_cache cache;
   hg_attention_call call;
-  float* partial;       // [2 per block][kHeadTile][head_dim + 2]: sums, maximum, sum of weights; null: no unit is split
-  Join* joins;          // [blocks]: the unit whose second part begins the block's share; parts 0: none
+  float* partial;       // LINE: [blocks][kHeadTile][head_dim + 2]: sums, maximum, sum of weights of a block's first part
+  uint64_t* tags;       // LINE: [blocks]
   int head_units;       // kv heads x chunks of kHeadTile heads
   int chunks, group;
+  int split;            // blocks of a unit: 1, 2, 4, 8 or 16
+  uint32_t page_tiles, by_page_tiles;   // tiles of a page, and ceil(2^32 / page_tiles)
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -61,7 +80,25 @@ __device__ __forceinline__ uint32_t half2_bits(float low, float high) {
   const __half2 h = __floats2half2_rn(low, high);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float scale_of(uint32_t word, int g) { return __uint_as_float(((word >> (8 * g)) & 255u) << 23); }
+// 2^(byte - 127) of byte g; 0 for byte 0.
+__device__ __forceinline__ float scale_of(uint32_t word, int g) { return __uint_as_float(__byte_perm(word, 0, 0x0444 | (g << 12)) >> 1); }
+__device__ __forceinline__ float power_of(int biased) { return __uint_as_float(uint32_t(biased) << 23); }
+
+__device__ __forceinline__ uint4 shared_16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 shared_8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t shared_4(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
 
 // Tiles that sequence i has to look at: from .. to - 1 hold positions first .. length - 1.
 struct Span { int first, length, from, to; };
@@ -123,95 +160,81 @@ __device__ __forceinline__ void write_out(const AttentionParams& p, int seq, int
   if (p.call.lse && d == 0) p.call.lse[int64_t(seq) * p.call.heads + head] = l == 0.f ? -INFINITY : (m - kBias + log2f(l)) * 0.69314718f;
 }
 
-// Results of one head unit.  `value(h, d)` gives the four weighted sums of head h from element d on.
-template <typename T, int GROUPS, typename Value, typename Weight, typename Maximum>
-__device__ __forceinline__ void finish(const AttentionParams& p, int seq, int head0, int heads, Value value, Weight weight, Maximum maximum) {
-  constexpr int kDim = 32 * GROUPS;
-  for (int i = threadIdx.x; i < heads * kDim / 4; i += kThreads) {   // whole groups of eight lanes
-    const int h = i / (kDim / 4), d = (i % (kDim / 4)) * 4;
-    write_out<T, GROUPS>(p, seq, head0 + h, d, value(h, d), weight(h), maximum(h));
+// Adds the sums of `count` other blocks, in their order, to m, l and sum; `load(j, sums, {maximum, weight})` for some of them together.
+template <typename Load>
+__device__ __forceinline__ void meet(int count, float& m, float& l, float4& sum, Load load) {
+  for (int first = 0; first < count; first += kMeet) {
+    float4 x[kMeet];
+    float2 y[kMeet];
+#pragma unroll
+    for (int j = 0; j < kMeet; ++j) load(min(first + j, count - 1), x[j], y[j]);
+    const float before = m;
+#pragma unroll
+    for (int j = 0; j < kMeet; ++j) m = fmaxf(m, y[j].x);
+    const float shrink = exp2_approx(before - m);
+    l *= shrink;
+    sum.x *= shrink; sum.y *= shrink; sum.z *= shrink; sum.w *= shrink;
+#pragma unroll
+    for (int j = 0; j < kMeet; ++j) {
+      if (first + j >= count) continue;
+      const float factor = exp2_approx(y[j].x - m);
+      l += y[j].y * factor;
+      sum.x += x[j].x * factor; sum.y += x[j].y * factor; sum.z += x[j].z * factor; sum.w += x[j].w * factor;
+    }
   }
 }
 
-__device__ __forceinline__ uint4 load_16(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 load_8(const uint8_t* p) {
-  uint2 v;
-  asm volatile("ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint32_t load_4(const uint8_t* p) {
-  uint32_t v;
-  asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(v) : "l"(p));
-  return v;
+// Waits until the tag is set; what was written before it is then visible.  False when it is not within about two seconds.
+__device__ __forceinline__ bool wait_for(const uint64_t* tag) {
+  const long long start = clock64();
+  for (uint32_t spin = 1;; ++spin) {
+    uint64_t now;
+    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(now) : "l"(tag) : "memory");
+    if (now == kTag) return true;
+    if ((spin & 63u) == 0) {
+      __nanosleep(100);
+      if (clock64() - start > kWaitLimitCycles) return false;
+    }
+  }
 }
 
-// A lane's part of one tile, as the fragments take it.
+// Shared memory of a block.  A tile of keys or values is 16 rows of head_dim bytes, whose 16-byte chunks the copy swizzles (with the
+// period of 128-byte rows, or of 64-byte ones).
 template <int GROUPS>
-struct Tile {
-  uint32_t k[2][2 * GROUPS];   // tokens r and r + 8: for the steps (g, j) the word [GROUPS j + g]
-  uint32_t v[4][GROUPS];       // tokens 2c, 2c + 1, 2c + 8, 2c + 9: elements 32 g + 4 r ...
-  uint32_t ks[2], vs[2];       // scale bytes of the groups, tokens r and r + 8
+struct Shared {
+  static constexpr int kDim = 32 * GROUPS, kCodes = kTile * kDim, kScales = kTile * 2 * GROUPS, kRow = kDim + 4;
+  static constexpr int kScalesAt = kWarps * kRing * 2 * kCodes, kSumsAt = kScalesAt + kWarps * kRing * kScales;
+  static constexpr int kBytes = kSumsAt + kWarps * kHeadTile * kRow * 4 + 1024;   // the beginning is brought to a multiple of 1024
 };
-
+// Row r of a fragment's eight holds this token: two rows that are read in one pass, r and r ^ 1, then have their chunks in different
+// banks, and so have the four tokens 2c that lanes read values of in one pass.
+__device__ __forceinline__ int token_of(int r) { return r ^ ((r & 1) << 2); }
+// Byte of a tile's 16-byte chunk.
 template <int GROUPS>
-__device__ __forceinline__ void load_keys(Tile<GROUPS>& t, const uint8_t* record, int page_size, int at, int r, int c) {
-  constexpr int kDim = 32 * GROUPS;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint8_t* const row = record + (at + r + 8 * i) * kDim + 16 * c;
-    const uint4 x = load_16(row);
-    t.k[i][0] = x.x; t.k[i][1] = x.y; t.k[i][2] = x.z; t.k[i][3] = x.w;
-    if constexpr (GROUPS == 4) {
-      const uint4 y = load_16(row + 64);
-      t.k[i][4] = y.x; t.k[i][5] = y.y; t.k[i][6] = y.z; t.k[i][7] = y.w;
-    }
-  }
-}
-template <int GROUPS>
-__device__ __forceinline__ void load_scales(uint32_t (&ks)[2], uint32_t (&vs)[2], const uint8_t* record, int page_size, int at, int r) {
-  const uint8_t* const scales = record + 2 * page_size * (32 * GROUPS);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint8_t* const s = scales + (at + r + 8 * i) * 2 * GROUPS;
-    if constexpr (GROUPS == 4) {
-      const uint2 x = load_8(s);
-      ks[i] = x.x; vs[i] = x.y;
-    } else {
-      const uint32_t x = load_4(s);
-      ks[i] = x & 0xffffu; vs[i] = x >> 16;
-    }
-  }
-}
-template <int GROUPS>
-__device__ __forceinline__ void load_values(Tile<GROUPS>& t, const uint8_t* record, int page_size, int at, int r, int c) {
-  constexpr int kDim = 32 * GROUPS;
-  const uint8_t* const values = record + page_size * kDim;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint8_t* const row = values + (at + 2 * c + (i & 1) + 8 * (i >> 1)) * kDim + 4 * GROUPS * r;
-    if constexpr (GROUPS == 4) {
-      const uint4 x = load_16(row);
-      t.v[i][0] = x.x; t.v[i][1] = x.y; t.v[i][2] = x.z; t.v[i][3] = x.w;
-    } else {
-      const uint2 x = load_8(row);
-      t.v[i][0] = x.x; t.v[i][1] = x.y;
-    }
-  }
+__device__ __forceinline__ uint32_t chunk_at(int token, int chunk) {
+  return uint32_t(token * 32 * GROUPS + ((chunk ^ (GROUPS == 4 ? token & 7 : (token >> 1) & 3)) << 4));
 }
 
-template <typename T, int GROUPS>
+template <typename T, int GROUPS, bool LINE>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
-attention_kernel(const AttentionParams p) {
-  constexpr int kDim = 32 * GROUPS, kSteps = 2 * GROUPS, kStride = kHeadTile * (kDim + 2);
-  __shared__ int64_t parts[kWarps], found_offset;
-  __shared__ int found_seq;
-  __shared__ alignas(16) float sums[kWarps][kHeadTile][kDim];   // four at a time
+attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ CUtensorMap map) {
+  using S = Shared<GROUPS>;
+  constexpr int kDim = 32 * GROUPS;
+  extern __shared__ uint8_t dynamic[];
+  __shared__ int given_up, there[kWarps][kRing];
   __shared__ float weights[kWarps][kHeadTile], maxima[kWarps][kHeadTile];
+  __shared__ alignas(8) float2 block_weights[kHeadTile];   // maximum and sum of weights of the block
+  __shared__ uint64_t full[kWarps][kRing];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u, bars = smem_u32(&full[warp][0]);
+  float (*const sums)[kHeadTile][S::kRow] = reinterpret_cast<float (*)[kHeadTile][S::kRow]>(dynamic + (base - smem_u32(dynamic)) + S::kSumsAt);
+  if (lane < kRing) mbar_init(bars + 8 * lane, 1);
+  if (threadIdx.x == 0) {
+    given_up = 0;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)) : "memory");
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
   // Loads below are ordinary ones: the kernel in front may still be writing the cache when this one starts, so the data is not
   // read-only for its duration.
   pdl_wait();
@@ -224,98 +247,130 @@ attention_kernel(const AttentionParams p) {
       *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.call.scales) + scale_word_offset(p.call.seqs + int(i / kblocks), int(i % kblocks), k)) = 0x7f7f7f7fu;
   }
 
-  // This block's share of the line: `remaining` from `offset` in the units of sequence `seq` on.
-  int seq;
-  int64_t offset, remaining, share = 0, position0 = 0;
-  if (p.partial) {
-    auto cost_of = [&](int i) -> int64_t {
-      if (i >= p.call.seqs) return 0;
+  // The block's units.
+  int seq, offset = 0;                     // LINE: `offset` in the units of sequence `seq`, `remaining` of its share of the line, `position` on it
+  int64_t remaining = 1, share = 1, position = 0;
+  int head_unit = 0, rank = 0;
+  if constexpr (LINE) {
+    __shared__ int64_t sums_of[kWarps];
+    __shared__ int found[2], largest_of[kWarps];
+    auto tiles_of = [&](int i) {
+      if (i >= p.call.seqs) return -kUnitCost;
       const Span s = span_of(p, i);
-      return int64_t(s.to - s.from + kUnitCost) * p.head_units;
+      return s.to - s.from;
     };
-    int64_t mine = cost_of(threadIdx.x), cost = mine;
-    for (int i = threadIdx.x + kThreads; i < p.call.seqs; i += kThreads) cost += cost_of(i);
-    Sums s = block_sums(cost, parts);
-    const int64_t all = s.all;
-    share = max(int64_t(kLeastShare), (all + gridDim.x - 1) / gridDim.x);
-    position0 = blockIdx.x * share;
-    remaining = min(share, all - position0);
-    if (remaining <= 0) {
-      if (threadIdx.x == 0) p.joins[blockIdx.x].parts = 0;
-      return;
+    const int tiles = tiles_of(threadIdx.x);
+    int largest = tiles;
+    int64_t mine = int64_t(tiles + kUnitCost) * p.head_units, cost = mine;
+    for (int i = threadIdx.x + kThreads; i < p.call.seqs; i += kThreads) {
+      const int other = tiles_of(i);
+      largest = max(largest, other);
+      cost += int64_t(other + kUnitCost) * p.head_units;
     }
-    if (p.call.seqs > kThreads) s = block_sums(mine, parts);
-    int64_t before = 0;
-    for (int base = 0;;) {
-      const int64_t end = before + s.upto;
-      if (position0 < end && position0 >= end - mine) {
-        found_seq = base + threadIdx.x;
-        found_offset = position0 - (end - mine);
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    if (lane == 0) largest_of[warp] = largest;
+    Sums s = block_sums(cost, sums_of);
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) largest = max(largest, largest_of[i]);
+    largest += kUnitCost;
+    share = max(int64_t(kLeastShare), (s.all + gridDim.x - 1) / gridDim.x);
+    const int64_t units = int64_t(p.call.seqs) * p.head_units;
+    if (units <= gridDim.x && largest * 4 <= share * 5) {
+      // As many blocks as units, and none much longer than a share: no unit is split.
+      if (blockIdx.x >= units) return;
+      seq = blockIdx.x / p.head_units;
+      const Span w = span_of(p, seq);
+      share = w.to - w.from + kUnitCost;
+      offset = int(blockIdx.x - seq * p.head_units) * int(share);
+      remaining = share;
+    } else {
+      position = blockIdx.x * share;
+      remaining = min(share, s.all - position);
+      if (remaining <= 0) return;
+      if (p.call.seqs > kThreads) s = block_sums(mine, sums_of);
+      int64_t before = 0;
+      for (int first = 0;;) {
+        const int64_t end = before + s.upto;
+        if (position < end && position >= end - mine) {
+          found[0] = first + threadIdx.x;
+          found[1] = int(position - (end - mine));
+        }
+        before += s.all;
+        first += kThreads;
+        if (first >= p.call.seqs || position < before) break;
+        mine = int64_t(tiles_of(first + threadIdx.x) + kUnitCost) * p.head_units;
+        s = block_sums(mine, sums_of);
       }
-      before += s.all;
-      base += kThreads;
-      if (base >= p.call.seqs || position0 < before) break;
-      mine = cost_of(base + threadIdx.x);
-      s = block_sums(mine, parts);
+      __syncthreads();
+      seq = found[0];
+      offset = found[1];
     }
-    __syncthreads();
-    seq = found_seq;
-    offset = found_offset;
   } else {
-    seq = blockIdx.x / p.head_units;
-    offset = blockIdx.x - seq * p.head_units;
-    remaining = 1;
+    const int unit = blockIdx.x / p.split;
+    rank = blockIdx.x - unit * p.split;
+    seq = unit / p.head_units;
+    head_unit = unit - seq * p.head_units;
   }
 
-  const int64_t record_bytes = cache_page_bytes(p.cache.page_size, kDim);
+  const int record_rows = p.cache.page_size * 2 + p.cache.page_size / 16;
+  auto place_of = [&](int t) { return int(p.page_tiles == 1 ? uint32_t(t) : __umulhi(uint32_t(t), p.by_page_tiles)); };
+  int copied = 0;                          // stage of the next copy
+  int stage = 0;
+  uint32_t phase = 0;
+  bool lost = false;   // a copy did not arrive: this warp's results become NaN
+  const int my_token = token_of(r), value_token = token_of(2 * c), odd_token = token_of(2 * c + 1);
+  const uint32_t key_at = chunk_at<GROUPS>(my_token, c);
+  const uint32_t value_at = GROUPS == 4 ? chunk_at<4>(value_token, r) : chunk_at<2>(value_token, r >> 1) + 8 * (r & 1);
+  const uint32_t odd_at = GROUPS == 4 ? chunk_at<4>(odd_token, r) : chunk_at<2>(odd_token, r >> 1) + 8 * (r & 1);
   for (bool first = true; remaining > 0; first = false) {
-    // The next unit, or this block's part of it.
     const Span span = span_of(p, seq);
-    const int tiles = span.to - span.from;
-    int head_unit = int(offset), begin = 0, end = tiles;
-    bool whole_unit = true;
-    if (p.partial) {
-      const int cost = tiles + kUnitCost;
-      head_unit = int(offset / cost);
-      const int from = int(offset - int64_t(head_unit) * cost), to = int(min(int64_t(cost), from + remaining));
-      begin = max(0, from - kUnitCost);
-      end = max(0, to - kUnitCost);
-      whole_unit = from == 0 && to == cost;
-      if (first && threadIdx.x == 0) {
-        // The second part of a unit is at the beginning of the block behind the one that holds the unit's beginning.
-        const int64_t unit0 = position0 - from, before = position0 - share;
-        Join j{seq, head_unit, 2 * int(blockIdx.x - 1) + (unit0 > before), 0};
-        if (from > 0 && unit0 >= before) j.parts = int((unit0 + cost - 1) / share) - int(blockIdx.x) + 2;
-        p.joins[blockIdx.x] = j;
-      }
-      remaining -= to - from;
-      offset += to - from;
+    int begin, end, from = 0, to = 0, cost = 0;   // tiles; LINE: the part of the unit's cost
+    if constexpr (LINE) {
+      cost = span.to - span.from + kUnitCost;
+      head_unit = int(uint32_t(offset) / uint32_t(cost));
+      from = offset - head_unit * cost;
+      to = int(min(int64_t(cost), from + remaining));
+      begin = span.from + max(0, from - kUnitCost);
+      end = span.from + max(0, to - kUnitCost);
     } else {
-      remaining = 0;
+      const int tiles = (span.to - span.from + p.split - 1) / p.split;
+      begin = min(span.to, span.from + rank * tiles);
+      end = min(span.to, begin + tiles);
     }
-    begin += span.from;
-    end += span.from;
     const int kv_head = head_unit / p.chunks, chunk = head_unit - kv_head * p.chunks;
     const int head0 = kv_head * p.group + chunk * kHeadTile, heads = min(kHeadTile, p.group - chunk * kHeadTile);
 
-    // The first tile, on its way while the queries are prepared.
+    // Copies run ahead of the tiles that are multiplied.  The number of the next tile's page is on its way a tile earlier.
     const int* const table = p.call.table + seq * p.call.table_stride;
-    const uint8_t* const head_data = static_cast<const uint8_t*>(p.cache.data) + kv_head * record_bytes;
-    auto page_of = [&](int t) { return t < end ? table[t * kTile / p.cache.page_size] : -1; };
-    // A page that is not there gives way to the first one, whose entries are then not used.
-    auto record_of = [&](int page) { return head_data + (uint32_t(page) < uint32_t(p.cache.pages) ? page : 0) * (record_bytes * p.cache.kv_heads); };
-    auto place_of = [&](int t) { return t * kTile % p.cache.page_size; };
-    int t = begin + warp, page = page_of(t), next_page = page_of(t + kWarps);
-    Tile<GROUPS> tile;
-    if (t < end) {
-      load_keys(tile, record_of(page), p.cache.page_size, place_of(t), r, c);
-      load_scales<GROUPS>(tile.ks, tile.vs, record_of(page), p.cache.page_size, place_of(t), r);
-      load_values(tile, record_of(page), p.cache.page_size, place_of(t), r, c);
-    }
+    int ahead_tile = begin + warp, ahead_page = ahead_tile < end ? table[place_of(ahead_tile)] : 0;
+    auto copy_next = [&] {
+      if (ahead_tile >= end) return;
+      const int next_page = ahead_tile + kWarps < end ? table[place_of(ahead_tile + kWarps)] : 0;
+      if (elect_one()) {
+        // A page that is not there gives way to the first one, whose entries are then not used.
+        const bool here = uint32_t(ahead_page) < uint32_t(p.cache.pages);
+        const int record = (here ? ahead_page : 0) * p.cache.kv_heads + kv_head;
+        const int entry = (ahead_tile - place_of(ahead_tile) * int(p.page_tiles)) * kTile, row = record * record_rows + entry;
+        const uint32_t bar = bars + 8 * copied, slot = uint32_t(warp * kRing + copied);
+        there[warp][copied] = here;
+        mbar_expect_tx(bar, 2 * S::kCodes + S::kScales);
+        tma_load_2d(base + slot * (2 * S::kCodes), &map, bar, 0, row);
+        tma_load_2d(base + slot * (2 * S::kCodes) + S::kCodes, &map, bar, 0, row + p.cache.page_size);
+        bulk_load(base + S::kScalesAt + slot * S::kScales,
+                  static_cast<const uint8_t*>(p.cache.data) + (int64_t(record) * record_rows + 2 * p.cache.page_size) * kDim + entry * 2 * GROUPS, S::kScales, bar);
+      }
+      __syncwarp();
+      copied = copied == kRing - 1 ? 0 : copied + 1;
+      ahead_tile += kWarps;
+      ahead_page = next_page;
+    };
+#pragma unroll 1
+    for (int i = 0; i < kRing - 1 && !lost; ++i) copy_next();
 
-    // Queries as the second operand: column r is head r, rows the four elements at 32 g + 4 x of step (g, j).
-    uint32_t q[kSteps][2];
-    float q_scale = 1.f;
+    // Queries as the second operand of the first product: column r is head r, rows the four elements at 32 g + 4 x.  A head's bf16 queries
+    // become halves under a power of two that brings the largest to [2^14, 2^15).
+    uint32_t q[GROUPS][2][2];
+    float to_log2[2];
     {
       const uint16_t* const row = static_cast<const uint16_t*>(p.call.q) + seq * p.call.q_stride + int64_t(head0 + r) * kDim;
       uint32_t top = 0;
@@ -324,27 +379,31 @@ attention_kernel(const AttentionParams p) {
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
           const int x = GROUPS == 4 ? 4 * j + c : 2 * c + j;
-          const uint2 w = r < heads ? *reinterpret_cast<const uint2*>(row + 32 * g + 4 * x) : make_uint2(0, 0);
-          q[GROUPS * j + g][0] = w.x;
-          q[GROUPS * j + g][1] = w.y;
-          top = max(max(top, max(w.x & 0x7fffu, (w.x >> 16) & 0x7fffu)), max(w.y & 0x7fffu, (w.y >> 16) & 0x7fffu));
+          const uint2 v = r < heads ? *reinterpret_cast<const uint2*>(row + 32 * g + 4 * x) : make_uint2(0, 0);
+          q[g][j][0] = v.x;
+          q[g][j][1] = v.y;
+          top = max(max(top, max(v.x & 0x7fffu, (v.x >> 16) & 0x7fffu)), max(v.y & 0x7fffu, (v.y >> 16) & 0x7fffu));
         }
+      float back = p.call.scale * 1.44269504f;
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        // One power of two brings the largest of the unit's queries to [2^14, 2^15).
-        top = __reduce_max_sync(0xffffffffu, top);
+#pragma unroll
+        for (int step = 1; step < 4; step <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, step));
         const int biased = min(253, max(1, 127 + 14 + 127 - int(top >> 7)));
-        const float factor = __uint_as_float(uint32_t(biased) << 23);
-        q_scale = __uint_as_float(uint32_t(254 - biased) << 23);
+        const float factor = power_of(biased);
+        back *= power_of(254 - biased);
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i)
+        for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 pair = Packed<T>::widen(q[i][h]);
-            q[i][h] = half2_bits(pair.x * factor, pair.y * factor);
-          }
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 pair = Packed<T>::widen(q[g][j][i]);
+              q[g][j][i] = half2_bits(pair.x * factor, pair.y * factor);
+            }
       }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) to_log2[h] = __shfl_sync(0xffffffffu, back, 8 * c + 4 * h);
     }
-    const float to_log2 = p.call.scale * 1.44269504f * q_scale;
 
     float out[GROUPS][2][4];
 #pragma unroll
@@ -353,127 +412,160 @@ attention_kernel(const AttentionParams p) {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) out[g][h][i] = 0.f;
-    float maximum[2] = {kNone, kNone}, weight[2] = {0.f, 0.f};   // heads 2c and 2c + 1; weights of this lane's tokens
-    int value_scale = 0;                                         // exponent byte under which values are summed
+    // Heads 2c and 2c + 1.  Weights (of this lane's tokens) and values are summed over 2^(maximum + value_scale - 127 - kBias).
+    float maximum[2] = {kNone, kNone}, weight[2] = {0.f, 0.f}, shift[2] = {-kNone, -kNone};
+    int value_scale = kLeastScale;
 
-    for (; t < end; t += kWarps) {
-      const int position = t * kTile;
-      const bool more = t + kWarps < end;
-      const int after = page_of(t + 2 * kWarps);
+    for (int t = begin + warp; t < end; t += kWarps) {
+      if (!lost && !warp_wait(bars + 8 * stage, phase, &given_up)) {
+        lost = true;
+        given_up = 1;
+      }
+      if (lost) continue;
+      const uint32_t slot = uint32_t(warp * kRing + stage), keys = base + slot * (2 * S::kCodes), values = keys + S::kCodes;
+      const uint32_t scales = base + S::kScalesAt + slot * S::kScales + uint32_t(my_token) * (2 * GROUPS);
       // Entries outside the span may hold anything: no score, no value and no scale of theirs is used.
-      const int to = uint32_t(page) < uint32_t(p.cache.pages) ? span.length : 0;
-      const bool whole = position >= span.first && position + kTile <= to;
+      const int first_position = t * kTile, length = there[warp][stage] ? span.length : 0;
+      const bool whole = first_position >= span.first && first_position + kTile <= length;
+      uint32_t k[2][2 * GROUPS], ks[2], vs[2];               // tokens my_token and my_token + 8
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < GROUPS / 2; ++j) {
+          const uint4 v = shared_16(keys + (key_at ^ (64 * j)) + i * 8 * kDim);
+          k[i][4 * j] = v.x; k[i][4 * j + 1] = v.y; k[i][4 * j + 2] = v.z; k[i][4 * j + 3] = v.w;
+        }
+        if constexpr (GROUPS == 4) {
+          const uint2 v = shared_8(scales + i * 16 * GROUPS);
+          ks[i] = v.x; vs[i] = v.y;
+        } else {
+          const uint32_t v = shared_4(scales + i * 16 * GROUPS);
+          ks[i] = v & 0xffffu; vs[i] = v >> 16;
+        }
+      }
       bool seen[2] = {true, true};
       if (!whole) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          seen[i] = position + r + 8 * i >= span.first && position + r + 8 * i < to;
-          if (!seen[i]) tile.ks[i] = tile.vs[i] = 0;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = position + 2 * c + (i & 1) + 8 * (i >> 1);
-          if (at < span.first || at >= to) {
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g) tile.v[i][g] = 0;
-          }
+          const int at_position = first_position + my_token + 8 * i;
+          seen[i] = at_position >= span.first && at_position < length;
+          if (!seen[i]) ks[i] = vs[i] = 0;
         }
       }
-      // Scores: tokens r and r + 8, heads 2c and 2c + 1.
+      // Scores: tokens my_token and my_token + 8, heads 2c and 2c + 1.
       float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int w = GROUPS * j + g;
-          mma_f16(part, e4m3x2_to_half2(uint16_t(tile.k[0][w])), e4m3x2_to_half2(uint16_t(tile.k[1][w])),
-                  e4m3x2_to_half2(uint16_t(tile.k[0][w] >> 16)), e4m3x2_to_half2(uint16_t(tile.k[1][w] >> 16)), q[w][0], q[w][1]);
+          const int i = GROUPS * j + g;
+          mma_f16(part, e4m3x2_to_half2(uint16_t(k[0][i])), e4m3x2_to_half2(uint16_t(k[1][i])),
+                  e4m3x2_to_half2(uint16_t(k[0][i] >> 16)), e4m3x2_to_half2(uint16_t(k[1][i] >> 16)), q[g][j][0], q[g][j][1]);
         }
-        const float low = scale_of(tile.ks[0], g), high = scale_of(tile.ks[1], g);
+        const float low = scale_of(ks[0], g), high = scale_of(ks[1], g);
         s[0] += low * part[0];
         s[1] += low * part[1];
         s[2] += high * part[2];
         s[3] += high * part[3];
       }
+      uint32_t v[4][GROUPS];                                 // tokens value_token, odd_token and those eight behind: elements 32 g + 4 r ...
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = seen[i >> 1] ? s[i] * to_log2 : -INFINITY;
-      // The next tile's keys take the place of these, as its values will.
-      const uint8_t* const next = record_of(next_page);
-      const int next_place = place_of(t + kWarps);
-      uint32_t next_ks[2] = {0, 0}, next_vs[2] = {0, 0};
-      if (more) {
-        load_keys(tile, next, p.cache.page_size, next_place, r, c);
-        load_scales<GROUPS>(next_ks, next_vs, next, p.cache.page_size, next_place, r);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t from = values + (i & 1 ? odd_at : value_at) + (i >> 1) * 8 * kDim;
+        if constexpr (GROUPS == 4) {
+          const uint4 u = shared_16(from);
+          v[i][0] = u.x; v[i][1] = u.y; v[i][2] = u.z; v[i][3] = u.w;
+        } else {
+          const uint2 u = shared_8(from);
+          v[i][0] = u.x; v[i][1] = u.y;
+        }
       }
+      // The tile before this one has been multiplied by all lanes; its stage takes the next copy.
+      __syncwarp();
+      copy_next();
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at_position = first_position + (i & 1 ? odd_token : value_token) + 8 * (i >> 1);
+          if (at_position < span.first || at_position >= length) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) v[i][g] = 0;
+          }
+        }
+      }
+      float x[4], scale[2][GROUPS], top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = seen[i >> 1] ? s[i] * to_log2[i & 1] + shift[i & 1] : -INFINITY;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) top = fmaxf(top, scale[i][g] = scale_of(vs[i], g));
 
       // A new maximum, or larger scales of the values, is taken up only when a weight could leave the range of a half.
-      const uint32_t tops = __vmaxu4(tile.vs[0], tile.vs[1]);
-      const int top = max(max(int(tops & 255), int((tops >> 8) & 255)), max(int((tops >> 16) & 255), int(tops >> 24)));
-      const bool rescale = fmaxf(s[0], s[2]) > maximum[0] + kSlack || fmaxf(s[1], s[3]) > maximum[1] + kSlack || top > value_scale + int(kSlack);
+      const bool rescale = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > float(127 - value_scale) + (kBias + kSlack) || top > power_of(value_scale) * 16.f;
       if (__any_sync(0xffffffffu, rescale)) {
-        const int new_scale = max(value_scale, __reduce_max_sync(0xffffffffu, top));
-        const float shrink = __uint_as_float(uint32_t(max(0, 127 + value_scale - new_scale)) << 23);
+        const int new_scale = max(value_scale, min(254, int(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23)));
+        const float shrink = power_of(max(0, 127 + value_scale - new_scale));
         value_scale = new_scale;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float m = fmaxf(s[h], s[h + 2]);
+          float m = fmaxf(seen[0] ? s[h] * to_log2[h] : kNone, seen[1] ? s[h + 2] * to_log2[h] : kNone);
 #pragma unroll
           for (int step = 4; step < 32; step <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, step));
           m = fmaxf(m, maximum[h]);
-          const float factor = exp2_approx(maximum[h] - m);
+          const float factor = exp2_approx(maximum[h] - m) * shrink;
           maximum[h] = m;
+          shift[h] = float(127 - value_scale) + kBias - m;
           weight[h] *= factor;
 #pragma unroll
-          for (int g = 0; g < GROUPS; ++g)
+          for (int i = 0; i < 2; ++i) {
+            x[h + 2 * i] = seen[i] ? s[h + 2 * i] * to_log2[h] + shift[h] : -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              out[g][i][h] *= factor * shrink;
-              out[g][i][h + 2] *= factor * shrink;
+            for (int g = 0; g < GROUPS; ++g) {
+              out[g][i][h] *= factor;
+              out[g][i][h + 2] *= factor;
             }
+          }
         }
       }
       float probability[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) probability[i] = exp2_approx(s[i] - maximum[i & 1] + kBias);
+      for (int i = 0; i < 4; ++i) probability[i] = exp2_approx(x[i]);
       weight[0] += probability[0] + probability[2];
       weight[1] += probability[1] + probability[3];
 
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
-        const float low = __uint_as_float(uint32_t(max(0, 127 + int((tile.vs[0] >> (8 * g)) & 255) - value_scale)) << 23);
-        const float high = __uint_as_float(uint32_t(max(0, 127 + int((tile.vs[1] >> (8 * g)) & 255) - value_scale)) << 23);
-        const uint32_t b0 = transpose8x8(half2_bits(probability[0] * low, probability[1] * low));
-        const uint32_t b1 = transpose8x8(half2_bits(probability[2] * high, probability[3] * high));
+        const uint32_t b0 = transpose8x8(half2_bits(probability[0] * scale[0][g], probability[1] * scale[0][g]));
+        const uint32_t b1 = transpose8x8(half2_bits(probability[2] * scale[1][g], probability[3] * scale[1][g]));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t near = __byte_perm(tile.v[0][g], tile.v[1][g], h ? 0x7362 : 0x5140), far = __byte_perm(tile.v[2][g], tile.v[3][g], h ? 0x7362 : 0x5140);
+          const uint32_t near = __byte_perm(v[0][g], v[1][g], h ? 0x7362 : 0x5140), far = __byte_perm(v[2][g], v[3][g], h ? 0x7362 : 0x5140);
           mma_f16(out[g][h], e4m3x2_to_half2(uint16_t(near)), e4m3x2_to_half2(uint16_t(near >> 16)),
                   e4m3x2_to_half2(uint16_t(far)), e4m3x2_to_half2(uint16_t(far >> 16)), b0, b1);
         }
       }
-      if (more) load_values(tile, next, p.cache.page_size, next_place, r, c);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        tile.ks[i] = next_ks[i];
-        tile.vs[i] = next_vs[i];
+      if (stage == kRing - 1) {
+        stage = 0;
+        phase ^= 1u;
+      } else {
+        ++stage;
       }
-      page = next_page;
-      next_page = after;
     }
 
     // The block's warps meet: sums under a common maximum.
-    if (!first) __syncthreads();   // the unit before has been read
+    if (!first) __syncthreads();   // those of the part before have been read
+    const float unit_scale = lost ? __uint_as_float(0x7fc00000u) : mx_scale(value_scale);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int step = 4; step < 32; step <<= 1) weight[h] += __shfl_xor_sync(0xffffffffu, weight[h], step);
       if (r == 0) {
-        weights[warp][2 * c + h] = weight[h];
+        weights[warp][2 * c + h] = weight[h] * unit_scale;
         maxima[warp][2 * c + h] = maximum[h];
       }
     }
-    const float unit_scale = mx_scale(value_scale);
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
@@ -481,93 +573,92 @@ attention_kernel(const AttentionParams p) {
         *reinterpret_cast<float4*>(&sums[warp][2 * c + h][32 * g + 4 * r]) =
             make_float4(out[g][0][h] * unit_scale, out[g][0][h + 2] * unit_scale, out[g][1][h] * unit_scale, out[g][1][h + 2] * unit_scale);
     __syncthreads();
-    auto block_maximum = [&](int h) {
-      float m = maxima[0][h];
+    const bool begins = from == 0, ends = to == cost;   // both, or CLUSTER: no other block of the line has a part
+    // Where the unit ends in a block behind this one, this block waits for the parts of the blocks up to there.
+    const int others = LINE && begins && !ends ? int((position + cost - 1) / share) - int(blockIdx.x) : 0;
+    if (others) {
+      for (int i = threadIdx.x; i < others; i += kThreads)
+        if (!wait_for(p.tags + blockIdx.x + 1 + i)) given_up = 1;
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < heads * kDim / 4; i += kThreads) {   // whole groups of eight lanes
+      const int h = i / (kDim / 4), d = (i % (kDim / 4)) * 4;
+      float m = maxima[0][h], l = 0.f;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) m = fmaxf(m, maxima[w][h]);
-      return m;
-    };
-    auto block_weight = [&](int h) {
-      const float m = block_maximum(h);
-      float l = 0.f;
+      for (int j = 1; j < kWarps; ++j) m = fmaxf(m, maxima[j][h]);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) l += weights[w][h] * exp2_approx(maxima[w][h] - m);
-      return l;
-    };
-    auto block_value = [&](int h, int d) {
-      const float m = block_maximum(h);
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float factor = exp2_approx(maxima[w][h] - m);
-        const float4 part = *reinterpret_cast<const float4*>(&sums[w][h][d]);
-        v.x += part.x * factor; v.y += part.y * factor; v.z += part.z * factor; v.w += part.w * factor;
+      for (int j = 0; j < kWarps; ++j) {
+        const float factor = exp2_approx(maxima[j][h] - m);
+        const float4 part = *reinterpret_cast<const float4*>(&sums[j][h][d]);
+        l += weights[j][h] * factor;
+        sum.x += part.x * factor; sum.y += part.y * factor; sum.z += part.z * factor; sum.w += part.w * factor;
       }
-      return v;
-    };
-    if (whole_unit) {
-      finish<T, GROUPS>(p, seq, head0, heads, block_value, block_weight, block_maximum);
+      if constexpr (LINE) {
+        constexpr int64_t kStride = kHeadTile * (kDim + 2);
+        if (!begins) {
+          float* const partial = p.partial + blockIdx.x * kStride;
+          *reinterpret_cast<float4*>(partial + h * kDim + d) = sum;
+          if (d == 0) *reinterpret_cast<float2*>(partial + kHeadTile * kDim + 2 * h) = make_float2(m, l);
+          continue;
+        }
+        const float* const partial = p.partial + (blockIdx.x + 1) * kStride;
+        meet(others, m, l, sum, [&](int j, float4& x, float2& y) {
+          x = __ldcg(reinterpret_cast<const float4*>(partial + j * kStride + h * kDim + d));
+          y = __ldcg(reinterpret_cast<const float2*>(partial + j * kStride + kHeadTile * kDim + 2 * h));
+        });
+        if (others && given_up) l = __uint_as_float(0x7fc00000u);
+        write_out<T, GROUPS>(p, seq, head0 + h, d, sum, l, m);
+      } else if (p.split == 1) {
+        write_out<T, GROUPS>(p, seq, head0 + h, d, sum, l, m);
+      } else {
+        *reinterpret_cast<float4*>(&sums[0][h][d]) = sum;   // read by this thread alone until here
+        if (d == 0) block_weights[h] = make_float2(m, l);
+      }
+    }
+    if constexpr (LINE) {
+      if (!begins) {
+        __syncthreads();
+        if (threadIdx.x == 0) asm volatile("fence.acq_rel.gpu;\n st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p.tags + blockIdx.x), "l"(kTag) : "memory");
+      } else if (others) {
+        for (int i = threadIdx.x; i < others; i += kThreads) p.tags[blockIdx.x + 1 + i] = 0;
+      }
+      remaining -= to - from;
+      offset += to - from;
+      position += to - from;
+      if (offset == cost * p.head_units) {
+        ++seq;
+        offset = 0;
+      }
     } else {
-      float* const partial = p.partial + (2 * int64_t(blockIdx.x) + !first) * kStride;
-      for (int i = threadIdx.x; i < heads * kDim / 4; i += kThreads) {
-        const int h = i / (kDim / 4), d = (i % (kDim / 4)) * 4;
-        *reinterpret_cast<float4*>(partial + h * kDim + d) = block_value(h, d);
-      }
-      if (threadIdx.x < kHeadTile) {
-        partial[kHeadTile * kDim + threadIdx.x] = block_maximum(threadIdx.x);
-        partial[kHeadTile * (kDim + 1) + threadIdx.x] = block_weight(threadIdx.x);
+      remaining = 0;
+      if (p.split > 1) {
+        // The cluster's blocks meet: each adds up its share of the columns over all blocks, in their order.
+        cluster_sync();
+        const int columns = kHeadTile * kDim / 4 / p.split, i = rank * columns + threadIdx.x;
+        if (threadIdx.x < columns && i < heads * kDim / 4) {   // whole groups of eight lanes
+          const int h = i / (kDim / 4), d = (i % (kDim / 4)) * 4;
+          const uint32_t sums_at = smem_u32(&sums[0][h][d]), weights_at = smem_u32(&block_weights[h]);
+          float m = kNone, l = 0.f;
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          meet(p.split, m, l, sum, [&](int j, float4& x, float2& y) {
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(map_to_rank(sums_at, uint32_t(j))) : "memory");
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(y.x), "=f"(y.y) : "r"(map_to_rank(weights_at, uint32_t(j))) : "memory");
+          });
+          write_out<T, GROUPS>(p, seq, head0 + h, d, sum, l, m);
+        }
+        cluster_sync();   // no block leaves while another may read its sums
       }
     }
-    if (p.partial && offset == int64_t(tiles + kUnitCost) * p.head_units) {
-      ++seq;
-      offset = 0;
-    }
   }
-}
-
-// Adds the parts of a split unit, in their order; a block for each of its heads.
-template <typename T, int GROUPS>
-__global__ void __launch_bounds__(kThreads)
-attention_join_kernel(const AttentionParams p) {
-  constexpr int kDim = 32 * GROUPS, kStride = kHeadTile * (kDim + 2), kLanes = kDim / 4, kTeams = kThreads / kLanes;
-  __shared__ float4 values[kTeams][kLanes];
-  pdl_trigger();
-  pdl_wait();
-  const Join j = p.joins[blockIdx.x];
-  if (j.parts == 0) return;
-  const int kv_head = j.head_unit / p.chunks, chunk = j.head_unit - kv_head * p.chunks, h = blockIdx.y;
-  if (h >= min(kHeadTile, p.group - chunk * kHeadTile)) return;
-  const int head = kv_head * p.group + chunk * kHeadTile + h;
-  auto part = [&](int i) { return p.partial + int64_t(i == 0 ? j.first : 2 * (j.first / 2 + i)) * kStride; };
-  const int lane = threadIdx.x & 31;
-  float m = kNone, l = 0.f;
-  for (int i = lane; i < j.parts; i += 32) m = fmaxf(m, part(i)[kHeadTile * kDim + h]);
-#pragma unroll
-  for (int step = 16; step; step >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, step));
-  for (int i = lane; i < j.parts; i += 32) l += part(i)[kHeadTile * (kDim + 1) + h] * exp2_approx(part(i)[kHeadTile * kDim + h] - m);
-#pragma unroll
-  for (int step = 16; step; step >>= 1) l += __shfl_xor_sync(0xffffffffu, l, step);
-  const int team = threadIdx.x / kLanes, d = (threadIdx.x % kLanes) * 4;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = team; i < j.parts; i += kTeams) {
-    const float factor = exp2_approx(part(i)[kHeadTile * kDim + h] - m);
-    const float4 x = *reinterpret_cast<const float4*>(part(i) + h * kDim + d);
-    v.x += x.x * factor; v.y += x.y * factor; v.z += x.z * factor; v.w += x.w * factor;
+  if (lost) {   // time for what is still on its way to shared memory
+    const long long start = clock64();
+    while (clock64() - start < 400000ll) __nanosleep(1000);
   }
-  values[team][d / 4] = v;
-  __syncthreads();
-  if (threadIdx.x >= kLanes) return;
-#pragma unroll
-  for (int i = 1; i < kTeams; ++i) {
-    const float4 x = values[i][d / 4];
-    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-  }
-  write_out<T, GROUPS>(p, j.seq, head, d, v, l, m);
 }
 
 // How a call is spread over the device.
-struct Split { int chunks, head_units, blocks; int64_t longest; bool join; };
+struct Split { int chunks, head_units, split; int64_t units; bool line; int blocks; };
 Split split_of(const hg_cache& c, int seqs, int heads, int table_width, int window) {
   static const int sms = [] {
     int device = 0, n = 148;
@@ -578,28 +669,73 @@ Split split_of(const hg_cache& c, int seqs, int heads, int table_width, int wind
     return n;
   }();
   Split s;
-  const int group = heads / c.kv_heads;
+  const int group = heads / c.kv_heads, slots = sms * kBlocksPerSm;
   s.chunks = (group + kHeadTile - 1) / kHeadTile;
   s.head_units = c.kv_heads * s.chunks;
-  s.longest = (int64_t(table_width) * c.page_size + kTile - 1) / kTile;
-  if (window) s.longest = std::min<int64_t>(s.longest, (int64_t(window) + 2 * kTile - 2) / kTile);
-  s.join = s.longest > kWhole;
-  const int64_t units = int64_t(seqs) * s.head_units;
-  s.blocks = int(s.join ? std::min<int64_t>(sms * kBlocksPerSm, (units * (s.longest + kUnitCost) + kLeastShare - 1) / kLeastShare) : units);
+  s.units = int64_t(seqs) * s.head_units;
+  int64_t longest = (int64_t(table_width) * c.page_size + kTile - 1) / kTile;
+  if (window) longest = std::min<int64_t>(longest, (int64_t(window) + 2 * kTile - 2) / kTile);
+  s.split = 1;
+  while (s.split < kMostSplit && s.units * s.split * 2 <= slots && longest > s.split * kWarps) s.split *= 2;
+  s.line = longest > kWhole && s.units * longest > kFew;
+  s.blocks = int(s.line ? std::min<int64_t>(slots, (s.units * (longest + kUnitCost) + kLeastShare - 1) / kLeastShare) : s.units * s.split);
   return s;
 }
 
 void validate_attention(const hg_cache& c, int seqs, int heads, int table_width, int window) {
   validate_cache(c);
+  // rows of head_dim bytes, which the copies count in 32 bits
+  if (int64_t(c.pages) * c.kv_heads * (c.page_size * 2 + c.page_size / 16) > 0x7fffffff) throw std::runtime_error("hg_attention: the cache has too many rows");
   if (seqs < 0 || heads <= 0 || heads % c.kv_heads) throw std::runtime_error("hg_attention: heads must be a multiple of kv_heads");
   if (table_width < 0 || window < 0 || int64_t(table_width) * c.page_size > (int64_t(1) << 30)) throw std::runtime_error("hg_attention: invalid table width or window");
-  if (int64_t(seqs) * heads > (1 << 30)) throw std::runtime_error("hg_attention: too many sequences in one call");
+  // a sequence's units are counted in 32 bits
+  if (int64_t(seqs) * heads > (1 << 26) || (int64_t(table_width) * c.page_size / kTile + kUnitCost + 1) * heads > 0x7fffffff) throw std::runtime_error("hg_attention: too much work for one call");
 }
 
-template <typename T, int GROUPS>
+// The cache as rows of head_dim bytes; a copy takes sixteen.
+CUtensorMap cache_map(const hg_cache& c) {
+  static const EncodeTiled encode = encode_tiled();
+  CUtensorMap map;
+  std::memset(&map, 0, sizeof(map));
+  const cuuint64_t dims[2] = {cuuint64_t(c.head_dim), cuuint64_t(c.pages) * c.kv_heads * (c.page_size * 2 + c.page_size / 16)};
+  const cuuint64_t strides[1] = {cuuint64_t(c.head_dim)};
+  const cuuint32_t box[2] = {cuuint32_t(c.head_dim), cuuint32_t(kTile)}, elem[2] = {1u, 1u};
+  const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.data, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed with code " + std::to_string(int(r)));
+  return map;
+}
+
+template <typename T, int GROUPS, bool LINE>
 void launch_attention(const AttentionParams& p, const Split& s, cudaStream_t stream) {
-  check(launch_kernel(attention_kernel<T, GROUPS>, dim3(unsigned(s.blocks)), dim3(kThreads), 0, stream, p), "attention");
-  if (s.join) check(launch_kernel(attention_join_kernel<T, GROUPS>, dim3(unsigned(s.blocks), unsigned(std::min(kHeadTile, p.group))), dim3(kThreads), 0, stream, p), "attention join");
+  constexpr int kBytes = Shared<GROUPS>::kBytes;
+  static std::once_flag once[64];   // limits of the function on each device
+  int device = 0;
+  check(cudaGetDevice(&device), "cudaGetDevice");
+  if (device < 0 || device >= 64) throw std::runtime_error("Device ordinals 0..63 are supported");
+  std::call_once(once[device], [] {
+    check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, LINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes), "attention");
+    check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, LINE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "attention");
+  });
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(unsigned(s.blocks));
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = kBytes;
+  config.stream = stream;
+  cudaLaunchAttribute attribute[2];
+  int count = 0;
+  if (!LINE && s.split > 1) {
+    attribute[count].id = cudaLaunchAttributeClusterDimension;
+    attribute[count++].val.clusterDim = {unsigned(s.split), 1u, 1u};
+  }
+  if (pdl_enabled()) {
+    attribute[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[count++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  config.attrs = attribute;
+  config.numAttrs = unsigned(count);
+  check(cudaLaunchKernelEx(&config, attention_kernel<T, GROUPS, LINE>, p, cache_map(p.cache)), "attention");
 }
 
 }  // namespace
@@ -612,8 +748,7 @@ int64_t hg_attention_workspace(const hg_cache* cache, int seqs, int heads, int t
     if (!cache) throw std::runtime_error("Null argument to hg_attention_workspace");
     hg::validate_attention(*cache, seqs, heads, table_width, window);
     const hg::Split s = hg::split_of(*cache, seqs, heads, table_width, window);
-    if (!s.join || !seqs) return 0;
-    return int64_t(s.blocks) * (sizeof(hg::Join) + 2 * hg::kHeadTile * (cache->head_dim + 2) * sizeof(float));
+    return !s.line || !seqs ? 0 : (s.blocks + 1 & ~1) * int64_t(sizeof(uint64_t)) + s.blocks * int64_t(hg::kHeadTile * (cache->head_dim + 2) * sizeof(float));
   } catch (std::exception const& e) {
     hg::last_error() = e.what();
     return -1;
@@ -634,15 +769,21 @@ int hg_attention(const hg_cache* cache, const hg_attention_call* call, int dtype
       reinterpret_cast<uintptr_t>(a.scales) % 16 || reinterpret_cast<uintptr_t>(a.workspace) % 16)
     throw std::runtime_error("hg_attention: pointers must be aligned to 16 bytes and q_stride to 8 elements");
   const hg::Split s = hg::split_of(*cache, a.seqs, a.heads, a.table_width, a.window);
-  if (s.join && !a.workspace) throw std::runtime_error("hg_attention: a workspace is needed");
-  hg::AttentionParams p{*cache, a, nullptr, nullptr, s.head_units, s.chunks, a.heads / cache->kv_heads};
-  if (s.join) {
-    p.joins = static_cast<hg::Join*>(a.workspace);
-    p.partial = reinterpret_cast<float*>(p.joins + s.blocks);
+  const uint32_t page_tiles = uint32_t(cache->page_size / hg::kTile);
+  hg::AttentionParams p{*cache, a, nullptr, nullptr, s.head_units, s.chunks, a.heads / cache->kv_heads, s.split, page_tiles,
+                        uint32_t(((uint64_t(1) << 32) + page_tiles - 1) / page_tiles)};
+  if (s.line) {
+    if (!a.workspace) throw std::runtime_error("hg_attention: a workspace is needed");
+    p.tags = static_cast<uint64_t*>(a.workspace);
+    p.partial = reinterpret_cast<float*>(p.tags + (s.blocks + 1 & ~1));
   }
   auto* const to = static_cast<cudaStream_t>(stream);
-  if (dtype == HG_DTYPE_BF16) cache->head_dim == 128 ? hg::launch_attention<__nv_bfloat16, 4>(p, s, to) : hg::launch_attention<__nv_bfloat16, 2>(p, s, to);
-  else cache->head_dim == 128 ? hg::launch_attention<__half, 4>(p, s, to) : hg::launch_attention<__half, 2>(p, s, to);
+  const bool bf16 = dtype == HG_DTYPE_BF16, wide = cache->head_dim == 128;
+  const auto launch = s.line ? (bf16 ? (wide ? hg::launch_attention<__nv_bfloat16, 4, true> : hg::launch_attention<__nv_bfloat16, 2, true>)
+                                     : (wide ? hg::launch_attention<__half, 4, true> : hg::launch_attention<__half, 2, true>))
+                             : (bf16 ? (wide ? hg::launch_attention<__nv_bfloat16, 4, false> : hg::launch_attention<__nv_bfloat16, 2, false>)
+                                     : (wide ? hg::launch_attention<__half, 4, false> : hg::launch_attention<__half, 2, false>));
+  launch(p, s, to);
   HG_CATCH
 }
 

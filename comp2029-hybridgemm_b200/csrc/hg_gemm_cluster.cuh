@@ -6,6 +6,12 @@
 
 namespace hg {
 
+// The driver's encoder of tensor maps, looked up once; throws where there is none.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled();
+
 struct ClusterPlan {
   int pair = 1;            // CTAs that share one MMA tile: 1, or 2 (cta_group::2)
   int split = 1;           // slices of K per tile, one CTA (pair) of the cluster each

@@ -934,11 +934,7 @@ Plan make_plan(int rows_low, int rows_high, int tokens, int k, int sms, int sche
 // Host side: tensor maps, handle, launch
 // ---------------------------------------------------------------------------------------------
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiled encode_tiled() {
+EncodeTiled encode_tiled() {
   static EncodeTiled fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {

@@ -4,7 +4,6 @@ import math
 import pytest
 import torch
 
-from hygemm_vllm import native
 from hygemm_vllm.cache import PagedCache, page_bytes
 
 pytestmark = pytest.mark.gpu
@@ -393,4 +392,3 @@ def test_refusals():
                            (data[:0], 16, 64), (data, 16, 96), (data, 0, 64), (data, 2048, 64)):
         with pytest.raises(ValueError):
             PagedCache(bad, page, dim)
-    assert native.library().hg_attention_workspace(cache._struct(), 1, 3, 1, 0) == -1
