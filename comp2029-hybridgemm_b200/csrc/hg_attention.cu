@@ -31,15 +31,14 @@ namespace {
 
 constexpr int kTile = 16;            // tokens of a step of one warp
 constexpr int kHeadTile = 8;         // query heads of a unit
-constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kBlocksPerSm = 3;
-constexpr int kRing = 3;             // tiles of a warp in shared memory or on their way there
+constexpr int kWarps = 4, kWideWarps = 12;   // of a block; of one that has an SM for itself
+constexpr int kBlocksPerSm = 4;      // of kWarps
+constexpr int kMostRing = 4;        // tiles of a warp in shared memory or on their way there, at most
 constexpr int kWhole = 16;           // sequences of no more tiles are not split
-constexpr int kUnitCost = 8;         // cost of a unit beside its tiles, in tiles
+constexpr int kUnitCost = 16;        // cost of a unit beside its tiles, in tiles
 constexpr int kLeastShare = 24;      // a block's share of the cost, where there is less for all blocks
 constexpr int kMostSplit = 16;       // blocks of a cluster at most
-constexpr int kFew = 8192;           // tiles of all units that are left to clusters
-constexpr int kMeet = 8;             // blocks whose sums are under way together
+constexpr int kSmBytes = 228 << 10;  // shared memory of an SM
 constexpr float kBias = 7.f, kSlack = 4.f;   // P is kept in [0, 2^(kBias + 2 kSlack)]
 constexpr float kNone = -1e30f;      // maximum of nothing
 constexpr int kLeastScale = 24;      // values are summed under 2^-103 at least
@@ -61,7 +60,8 @@ struct AttentionParams {
   uint64_t* tags;       // LINE: [blocks]
   int head_units;       // kv heads x chunks of kHeadTile heads
   int chunks, group;
-  int split;            // blocks of a unit: 1, 2, 4, 8 or 16
+  int split;            // CLUSTER: blocks of a unit, 1, 2, 4, 8 or 16
+  int ring;             // tiles of a warp in shared memory or on their way there
   uint32_t page_tiles, by_page_tiles;   // tiles of a page, and ceil(2^32 / page_tiles)
 };
 
@@ -113,6 +113,7 @@ __device__ __forceinline__ Span span_of(const AttentionParams& p, int i) {
 
 // Sums of what the block's threads give, of all and of those up to this one.
 struct Sums { int64_t all, upto; };
+template <int WARPS>
 __device__ __forceinline__ Sums block_sums(int64_t v, int64_t* parts) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -125,7 +126,7 @@ __device__ __forceinline__ Sums block_sums(int64_t v, int64_t* parts) {
   __syncthreads();
   Sums s{0, v};
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
+  for (int i = 0; i < WARPS; ++i) {
     if (i < warp) s.upto += parts[i];
     s.all += parts[i];
   }
@@ -161,7 +162,7 @@ __device__ __forceinline__ void write_out(const AttentionParams& p, int seq, int
 }
 
 // Adds the sums of `count` other blocks, in their order, to m, l and sum; `load(j, sums, {maximum, weight})` for some of them together.
-template <typename Load>
+template <int kMeet, typename Load>
 __device__ __forceinline__ void meet(int count, float& m, float& l, float4& sum, Load load) {
   for (int first = 0; first < count; first += kMeet) {
     float4 x[kMeet];
@@ -199,12 +200,14 @@ __device__ __forceinline__ bool wait_for(const uint64_t* tag) {
 }
 
 // Shared memory of a block.  A tile of keys or values is 16 rows of head_dim bytes, whose 16-byte chunks the copy swizzles (with the
-// period of 128-byte rows, or of 64-byte ones).
-template <int GROUPS>
+// period of 128-byte rows, or of 64-byte ones).  The warps' sums take the place of the rings when these are idle.
+template <int GROUPS, int WARPS>
 struct Shared {
   static constexpr int kDim = 32 * GROUPS, kCodes = kTile * kDim, kScales = kTile * 2 * GROUPS, kRow = kDim + 4;
-  static constexpr int kScalesAt = kWarps * kRing * 2 * kCodes, kSumsAt = kScalesAt + kWarps * kRing * kScales;
-  static constexpr int kBytes = kSumsAt + kWarps * kHeadTile * kRow * 4 + 1024;   // the beginning is brought to a multiple of 1024
+  static constexpr int kStage = 2 * kCodes + kScales;   // of a warp
+  static int bytes(int ring) {
+    return std::max(WARPS * ring * kStage, WARPS * kHeadTile * kRow * 4) + 1024;   // the beginning is brought to a multiple of 1024
+  }
 };
 // Row r of a fragment's eight holds this token: two rows that are read in one pass, r and r ^ 1, then have their chunks in different
 // banks, and so have the four tokens 2c that lanes read values of in one pass.
@@ -215,20 +218,21 @@ __device__ __forceinline__ uint32_t chunk_at(int token, int chunk) {
   return uint32_t(token * 32 * GROUPS + ((chunk ^ (GROUPS == 4 ? token & 7 : (token >> 1) & 3)) << 4));
 }
 
-template <typename T, int GROUPS, bool LINE>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+template <typename T, int GROUPS, int WARPS, bool LINE>
+__global__ void __launch_bounds__(WARPS * 32, WARPS == kWarps ? kBlocksPerSm : 1)
 attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ CUtensorMap map) {
-  using S = Shared<GROUPS>;
-  constexpr int kDim = 32 * GROUPS;
+  using S = Shared<GROUPS, WARPS>;
+  constexpr int kDim = 32 * GROUPS, kThreads = WARPS * 32;
   extern __shared__ uint8_t dynamic[];
-  __shared__ int given_up, there[kWarps][kRing];
-  __shared__ float weights[kWarps][kHeadTile], maxima[kWarps][kHeadTile];
+  __shared__ int given_up, there[WARPS][kMostRing];
+  __shared__ float weights[WARPS][kHeadTile], maxima[WARPS][kHeadTile];
   __shared__ alignas(8) float2 block_weights[kHeadTile];   // maximum and sum of weights of the block
-  __shared__ uint64_t full[kWarps][kRing];
+  __shared__ uint64_t full[WARPS][kMostRing];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u, bars = smem_u32(&full[warp][0]);
-  float (*const sums)[kHeadTile][S::kRow] = reinterpret_cast<float (*)[kHeadTile][S::kRow]>(dynamic + (base - smem_u32(dynamic)) + S::kSumsAt);
-  if (lane < kRing) mbar_init(bars + 8 * lane, 1);
+  const int ring = p.ring;
+  const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u, all_scales = base + uint32_t(WARPS * ring) * (2 * S::kCodes), bars = smem_u32(&full[warp][0]);
+  float (*const sums)[kHeadTile][S::kRow] = reinterpret_cast<float (*)[kHeadTile][S::kRow]>(dynamic + (base - smem_u32(dynamic)));
+  if (lane < p.ring) mbar_init(bars + 8 * lane, 1);
   if (threadIdx.x == 0) {
     given_up = 0;
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)) : "memory");
@@ -251,9 +255,10 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   int seq, offset = 0;                     // LINE: `offset` in the units of sequence `seq`, `remaining` of its share of the line, `position` on it
   int64_t remaining = 1, share = 1, position = 0;
   int head_unit = 0, rank = 0;
+  bool whole = !LINE;                      // whole units, every gridDim.x-th from this block's on
   if constexpr (LINE) {
-    __shared__ int64_t sums_of[kWarps];
-    __shared__ int found[2], largest_of[kWarps];
+    __shared__ int64_t sums_of[WARPS];
+    __shared__ int found[2], largest_of[WARPS];
     auto tiles_of = [&](int i) {
       if (i >= p.call.seqs) return -kUnitCost;
       const Span s = span_of(p, i);
@@ -269,25 +274,22 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     }
     largest = __reduce_max_sync(0xffffffffu, largest);
     if (lane == 0) largest_of[warp] = largest;
-    Sums s = block_sums(cost, sums_of);
+    Sums s = block_sums<WARPS>(cost, sums_of);
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) largest = max(largest, largest_of[i]);
+    for (int i = 0; i < WARPS; ++i) largest = max(largest, largest_of[i]);
     largest += kUnitCost;
     share = max(int64_t(kLeastShare), (s.all + gridDim.x - 1) / gridDim.x);
     const int64_t units = int64_t(p.call.seqs) * p.head_units;
-    if (units <= gridDim.x && largest * 4 <= share * 5) {
-      // As many blocks as units, and none much longer than a share: no unit is split.
+    whole = units * largest * 4 <= s.all * 5;
+    if (whole) {
+      // None much longer than the others: no unit is split.
       if (blockIdx.x >= units) return;
-      seq = blockIdx.x / p.head_units;
-      const Span w = span_of(p, seq);
-      share = w.to - w.from + kUnitCost;
-      offset = int(blockIdx.x - seq * p.head_units) * int(share);
-      remaining = share;
+      remaining = units - blockIdx.x;   // units
     } else {
       position = blockIdx.x * share;
       remaining = min(share, s.all - position);
       if (remaining <= 0) return;
-      if (p.call.seqs > kThreads) s = block_sums(mine, sums_of);
+      if (p.call.seqs > kThreads) s = block_sums<WARPS>(mine, sums_of);
       int64_t before = 0;
       for (int first = 0;;) {
         const int64_t end = before + s.upto;
@@ -299,18 +301,15 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
         first += kThreads;
         if (first >= p.call.seqs || position < before) break;
         mine = int64_t(tiles_of(first + threadIdx.x) + kUnitCost) * p.head_units;
-        s = block_sums(mine, sums_of);
+        s = block_sums<WARPS>(mine, sums_of);
       }
       __syncthreads();
       seq = found[0];
       offset = found[1];
     }
-  } else {
-    const int unit = blockIdx.x / p.split;
-    rank = blockIdx.x - unit * p.split;
-    seq = unit / p.head_units;
-    head_unit = unit - seq * p.head_units;
   }
+  int unit = LINE ? blockIdx.x : blockIdx.x / p.split;
+  if constexpr (!LINE) rank = blockIdx.x - unit * p.split;
 
   const int record_rows = p.cache.page_size * 2 + p.cache.page_size / 16;
   auto place_of = [&](int t) { return int(p.page_tiles == 1 ? uint32_t(t) : __umulhi(uint32_t(t), p.by_page_tiles)); };
@@ -322,16 +321,23 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   const uint32_t key_at = chunk_at<GROUPS>(my_token, c);
   const uint32_t value_at = GROUPS == 4 ? chunk_at<4>(value_token, r) : chunk_at<2>(value_token, r >> 1) + 8 * (r & 1);
   const uint32_t odd_at = GROUPS == 4 ? chunk_at<4>(odd_token, r) : chunk_at<2>(odd_token, r >> 1) + 8 * (r & 1);
-  for (bool first = true; remaining > 0; first = false) {
+  while (remaining > 0) {
+    if (whole) {
+      seq = unit / p.head_units;
+      head_unit = unit - seq * p.head_units;
+    }
     const Span span = span_of(p, seq);
-    int begin, end, from = 0, to = 0, cost = 0;   // tiles; LINE: the part of the unit's cost
-    if constexpr (LINE) {
+    int begin, end, from = 0, to = 0, cost = 0;   // tiles; the part of the unit's cost
+    if (!whole) {
       cost = span.to - span.from + kUnitCost;
       head_unit = int(uint32_t(offset) / uint32_t(cost));
       from = offset - head_unit * cost;
       to = int(min(int64_t(cost), from + remaining));
       begin = span.from + max(0, from - kUnitCost);
       end = span.from + max(0, to - kUnitCost);
+    } else if (LINE) {
+      begin = span.from;
+      end = span.to;
     } else {
       const int tiles = (span.to - span.from + p.split - 1) / p.split;
       begin = min(span.to, span.from + rank * tiles);
@@ -345,27 +351,27 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     int ahead_tile = begin + warp, ahead_page = ahead_tile < end ? table[place_of(ahead_tile)] : 0;
     auto copy_next = [&] {
       if (ahead_tile >= end) return;
-      const int next_page = ahead_tile + kWarps < end ? table[place_of(ahead_tile + kWarps)] : 0;
+      const int next_page = ahead_tile + WARPS < end ? table[place_of(ahead_tile + WARPS)] : 0;
       if (elect_one()) {
         // A page that is not there gives way to the first one, whose entries are then not used.
         const bool here = uint32_t(ahead_page) < uint32_t(p.cache.pages);
         const int record = (here ? ahead_page : 0) * p.cache.kv_heads + kv_head;
         const int entry = (ahead_tile - place_of(ahead_tile) * int(p.page_tiles)) * kTile, row = record * record_rows + entry;
-        const uint32_t bar = bars + 8 * copied, slot = uint32_t(warp * kRing + copied);
+        const uint32_t bar = bars + 8 * copied, slot = uint32_t(warp * ring + copied);
         there[warp][copied] = here;
         mbar_expect_tx(bar, 2 * S::kCodes + S::kScales);
         tma_load_2d(base + slot * (2 * S::kCodes), &map, bar, 0, row);
         tma_load_2d(base + slot * (2 * S::kCodes) + S::kCodes, &map, bar, 0, row + p.cache.page_size);
-        bulk_load(base + S::kScalesAt + slot * S::kScales,
+        bulk_load(all_scales + slot * S::kScales,
                   static_cast<const uint8_t*>(p.cache.data) + (int64_t(record) * record_rows + 2 * p.cache.page_size) * kDim + entry * 2 * GROUPS, S::kScales, bar);
       }
       __syncwarp();
-      copied = copied == kRing - 1 ? 0 : copied + 1;
-      ahead_tile += kWarps;
+      copied = copied == ring - 1 ? 0 : copied + 1;
+      ahead_tile += WARPS;
       ahead_page = next_page;
     };
 #pragma unroll 1
-    for (int i = 0; i < kRing - 1 && !lost; ++i) copy_next();
+    for (int i = 0; i < ring - 1 && !lost; ++i) copy_next();
 
     // Queries as the second operand of the first product: column r is head r, rows the four elements at 32 g + 4 x.  A head's bf16 queries
     // become halves under a power of two that brings the largest to [2^14, 2^15).
@@ -416,14 +422,14 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     float maximum[2] = {kNone, kNone}, weight[2] = {0.f, 0.f}, shift[2] = {-kNone, -kNone};
     int value_scale = kLeastScale;
 
-    for (int t = begin + warp; t < end; t += kWarps) {
+    for (int t = begin + warp; t < end; t += WARPS) {
       if (!lost && !warp_wait(bars + 8 * stage, phase, &given_up)) {
         lost = true;
         given_up = 1;
       }
       if (lost) continue;
-      const uint32_t slot = uint32_t(warp * kRing + stage), keys = base + slot * (2 * S::kCodes), values = keys + S::kCodes;
-      const uint32_t scales = base + S::kScalesAt + slot * S::kScales + uint32_t(my_token) * (2 * GROUPS);
+      const uint32_t slot = uint32_t(warp * ring + stage), keys = base + slot * (2 * S::kCodes), values = keys + S::kCodes;
+      const uint32_t scales = all_scales + slot * S::kScales + uint32_t(my_token) * (2 * GROUPS);
       // Entries outside the span may hold anything: no score, no value and no scale of theirs is used.
       const int first_position = t * kTile, length = there[warp][stage] ? span.length : 0;
       const bool whole = first_position >= span.first && first_position + kTile <= length;
@@ -546,7 +552,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
                   e4m3x2_to_half2(uint16_t(far)), e4m3x2_to_half2(uint16_t(far >> 16)), b0, b1);
         }
       }
-      if (stage == kRing - 1) {
+      if (stage == ring - 1) {
         stage = 0;
         phase ^= 1u;
       } else {
@@ -555,7 +561,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     }
 
     // The block's warps meet: sums under a common maximum.
-    if (!first) __syncthreads();   // those of the part before have been read
+    __syncthreads();   // the rings are idle
     const float unit_scale = lost ? __uint_as_float(0x7fc00000u) : mx_scale(value_scale);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -573,7 +579,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
         *reinterpret_cast<float4*>(&sums[warp][2 * c + h][32 * g + 4 * r]) =
             make_float4(out[g][0][h] * unit_scale, out[g][0][h + 2] * unit_scale, out[g][1][h] * unit_scale, out[g][1][h + 2] * unit_scale);
     __syncthreads();
-    const bool begins = from == 0, ends = to == cost;   // both, or CLUSTER: no other block of the line has a part
+    const bool begins = from == 0, ends = to == cost;   // whole units: both
     // Where the unit ends in a block behind this one, this block waits for the parts of the blocks up to there.
     const int others = LINE && begins && !ends ? int((position + cost - 1) / share) - int(blockIdx.x) : 0;
     if (others) {
@@ -586,9 +592,9 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       float m = maxima[0][h], l = 0.f;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int j = 1; j < kWarps; ++j) m = fmaxf(m, maxima[j][h]);
+      for (int j = 1; j < WARPS; ++j) m = fmaxf(m, maxima[j][h]);
 #pragma unroll
-      for (int j = 0; j < kWarps; ++j) {
+      for (int j = 0; j < WARPS; ++j) {
         const float factor = exp2_approx(maxima[j][h] - m);
         const float4 part = *reinterpret_cast<const float4*>(&sums[j][h][d]);
         l += weights[j][h] * factor;
@@ -603,7 +609,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
           continue;
         }
         const float* const partial = p.partial + (blockIdx.x + 1) * kStride;
-        meet(others, m, l, sum, [&](int j, float4& x, float2& y) {
+        meet<16>(others, m, l, sum, [&](int j, float4& x, float2& y) {
           x = __ldcg(reinterpret_cast<const float4*>(partial + j * kStride + h * kDim + d));
           y = __ldcg(reinterpret_cast<const float2*>(partial + j * kStride + kHeadTile * kDim + 2 * h));
         });
@@ -623,25 +629,34 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       } else if (others) {
         for (int i = threadIdx.x; i < others; i += kThreads) p.tags[blockIdx.x + 1 + i] = 0;
       }
-      remaining -= to - from;
-      offset += to - from;
-      position += to - from;
-      if (offset == cost * p.head_units) {
-        ++seq;
-        offset = 0;
+      if (whole) {
+        remaining -= gridDim.x;
+        unit += gridDim.x;
+      } else {
+        remaining -= to - from;
+        offset += to - from;
+        position += to - from;
+        if (offset == cost * p.head_units) {
+          ++seq;
+          offset = 0;
+        }
+      }
+      if (remaining > 0) {   // the sums have been read, and copies may take their place
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
       }
     } else {
       remaining = 0;
       if (p.split > 1) {
         // The cluster's blocks meet: each adds up its share of the columns over all blocks, in their order.
         cluster_sync();
-        const int columns = kHeadTile * kDim / 4 / p.split, i = rank * columns + threadIdx.x;
+        const int columns = kHeadTile * kDim / 4 / p.split, i = rank * columns + threadIdx.x;   // at least two blocks, 128 threads
         if (threadIdx.x < columns && i < heads * kDim / 4) {   // whole groups of eight lanes
           const int h = i / (kDim / 4), d = (i % (kDim / 4)) * 4;
           const uint32_t sums_at = smem_u32(&sums[0][h][d]), weights_at = smem_u32(&block_weights[h]);
           float m = kNone, l = 0.f;
           float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-          meet(p.split, m, l, sum, [&](int j, float4& x, float2& y) {
+          meet<8>(p.split, m, l, sum, [&](int j, float4& x, float2& y) {
             asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(map_to_rank(sums_at, uint32_t(j))) : "memory");
             asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(y.x), "=f"(y.y) : "r"(map_to_rank(weights_at, uint32_t(j))) : "memory");
           });
@@ -657,8 +672,8 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   }
 }
 
-// How a call is spread over the device.
-struct Split { int chunks, head_units, split; int64_t units; bool line; int blocks; };
+// How a call is spread over the device: blocks with an SM each in clusters of `split`, or a line (or whole units where sequences are short).
+struct Split { int chunks, head_units, split; int64_t units; bool wide, line; int blocks, ring; };
 Split split_of(const hg_cache& c, int seqs, int heads, int table_width, int window) {
   static const int sms = [] {
     int device = 0, n = 148;
@@ -669,16 +684,21 @@ Split split_of(const hg_cache& c, int seqs, int heads, int table_width, int wind
     return n;
   }();
   Split s;
-  const int group = heads / c.kv_heads, slots = sms * kBlocksPerSm;
+  const int group = heads / c.kv_heads;
   s.chunks = (group + kHeadTile - 1) / kHeadTile;
   s.head_units = c.kv_heads * s.chunks;
   s.units = int64_t(seqs) * s.head_units;
   int64_t longest = (int64_t(table_width) * c.page_size + kTile - 1) / kTile;
   if (window) longest = std::min<int64_t>(longest, (int64_t(window) + 2 * kTile - 2) / kTile);
+  s.wide = s.units <= sms && longest > kWhole;
+  s.line = !s.wide && longest > kWhole;
   s.split = 1;
-  while (s.split < kMostSplit && s.units * s.split * 2 <= slots && longest > s.split * kWarps) s.split *= 2;
-  s.line = longest > kWhole && s.units * longest > kFew;
-  s.blocks = int(s.line ? std::min<int64_t>(slots, (s.units * (longest + kUnitCost) + kLeastShare - 1) / kLeastShare) : s.units * s.split);
+  while (s.wide && s.split < kMostSplit && s.units * s.split * 2 <= sms && longest > s.split * kWideWarps) s.split *= 2;
+  s.blocks = int(s.line ? std::min<int64_t>(sms * kBlocksPerSm, (s.units * (longest + kUnitCost) + kLeastShare - 1) / kLeastShare) : s.units * s.split);
+  // As deep a ring as the blocks of an SM have room for, and use.
+  const int per_sm = s.wide ? 1 : kBlocksPerSm, warps = s.wide ? kWideWarps : kWarps;
+  const int room = (kSmBytes / per_sm - 2048) / (warps * (c.head_dim == 128 ? Shared<4, kWarps>::kStage : Shared<2, kWarps>::kStage));
+  s.ring = std::max(2, std::min({kMostRing, room, int((longest / s.split + warps - 1) / warps) + 1}));
   return s;
 }
 
@@ -707,21 +727,21 @@ CUtensorMap cache_map(const hg_cache& c) {
   return map;
 }
 
-template <typename T, int GROUPS, bool LINE>
+template <typename T, int GROUPS, int WARPS, bool LINE>
 void launch_attention(const AttentionParams& p, const Split& s, cudaStream_t stream) {
-  constexpr int kBytes = Shared<GROUPS>::kBytes;
+  const int bytes = Shared<GROUPS, WARPS>::bytes(s.ring);
   static std::once_flag once[64];   // limits of the function on each device
   int device = 0;
   check(cudaGetDevice(&device), "cudaGetDevice");
   if (device < 0 || device >= 64) throw std::runtime_error("Device ordinals 0..63 are supported");
   std::call_once(once[device], [] {
-    check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, LINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes), "attention");
-    check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, LINE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "attention");
+    check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, WARPS, LINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shared<GROUPS, WARPS>::bytes(kMostRing)), "attention");
+    check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, WARPS, LINE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "attention");
   });
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(unsigned(s.blocks));
-  config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = kBytes;
+  config.blockDim = dim3(WARPS * 32);
+  config.dynamicSmemBytes = size_t(bytes);
   config.stream = stream;
   cudaLaunchAttribute attribute[2];
   int count = 0;
@@ -735,7 +755,7 @@ void launch_attention(const AttentionParams& p, const Split& s, cudaStream_t str
   }
   config.attrs = attribute;
   config.numAttrs = unsigned(count);
-  check(cudaLaunchKernelEx(&config, attention_kernel<T, GROUPS, LINE>, p, cache_map(p.cache)), "attention");
+  check(cudaLaunchKernelEx(&config, attention_kernel<T, GROUPS, WARPS, LINE>, p, cache_map(p.cache)), "attention");
 }
 
 }  // namespace
@@ -770,7 +790,7 @@ int hg_attention(const hg_cache* cache, const hg_attention_call* call, int dtype
     throw std::runtime_error("hg_attention: pointers must be aligned to 16 bytes and q_stride to 8 elements");
   const hg::Split s = hg::split_of(*cache, a.seqs, a.heads, a.table_width, a.window);
   const uint32_t page_tiles = uint32_t(cache->page_size / hg::kTile);
-  hg::AttentionParams p{*cache, a, nullptr, nullptr, s.head_units, s.chunks, a.heads / cache->kv_heads, s.split, page_tiles,
+  hg::AttentionParams p{*cache, a, nullptr, nullptr, s.head_units, s.chunks, a.heads / cache->kv_heads, s.split, s.ring, page_tiles,
                         uint32_t(((uint64_t(1) << 32) + page_tiles - 1) / page_tiles)};
   if (s.line) {
     if (!a.workspace) throw std::runtime_error("hg_attention: a workspace is needed");
@@ -778,11 +798,15 @@ int hg_attention(const hg_cache* cache, const hg_attention_call* call, int dtype
     p.partial = reinterpret_cast<float*>(p.tags + (s.blocks + 1 & ~1));
   }
   auto* const to = static_cast<cudaStream_t>(stream);
-  const bool bf16 = dtype == HG_DTYPE_BF16, wide = cache->head_dim == 128;
-  const auto launch = s.line ? (bf16 ? (wide ? hg::launch_attention<__nv_bfloat16, 4, true> : hg::launch_attention<__nv_bfloat16, 2, true>)
-                                     : (wide ? hg::launch_attention<__half, 4, true> : hg::launch_attention<__half, 2, true>))
-                             : (bf16 ? (wide ? hg::launch_attention<__nv_bfloat16, 4, false> : hg::launch_attention<__nv_bfloat16, 2, false>)
-                                     : (wide ? hg::launch_attention<__half, 4, false> : hg::launch_attention<__half, 2, false>));
+  const auto pick = [&](auto type, auto groups) {
+    using T = decltype(type);
+    constexpr int G = decltype(groups)::value;
+    return s.wide ? hg::launch_attention<T, G, hg::kWideWarps, false> : s.line ? hg::launch_attention<T, G, hg::kWarps, true> : hg::launch_attention<T, G, hg::kWarps, false>;
+  };
+  using Two = std::integral_constant<int, 2>;
+  using Four = std::integral_constant<int, 4>;
+  const bool wide = cache->head_dim == 128;
+  const auto launch = dtype == HG_DTYPE_BF16 ? (wide ? pick(__nv_bfloat16{}, Four{}) : pick(__nv_bfloat16{}, Two{})) : (wide ? pick(__half{}, Four{}) : pick(__half{}, Two{}));
   launch(p, s, to);
   HG_CATCH
 }
