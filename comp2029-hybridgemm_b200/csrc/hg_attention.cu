@@ -32,12 +32,15 @@ namespace {
 constexpr int kTile = 16;            // tokens of a step of one warp
 constexpr int kHeadTile = 8;         // query heads of a unit
 constexpr int kWarps = 4, kWideWarps = 12;   // of a block; of one that has an SM for itself
-constexpr int kBlocksPerSm = 4;      // of kWarps
 constexpr int kMostRing = 4;        // tiles of a warp in shared memory or on their way there, at most
+constexpr int kBlocksPerSm = 4, kLineBlocksPerSm = 3;   // of kWarps; of a line of no more units than that
 constexpr int kWhole = 16;           // sequences of no more tiles are not split
 constexpr int kUnitCost = 16;        // cost of a unit beside its tiles, in tiles
 constexpr int kLeastShare = 24;      // a block's share of the cost, where there is less for all blocks
-constexpr int kMostSplit = 16;       // blocks of a cluster at most
+constexpr int kFew = 12288;          // tiles of all units that are left to clusters, whatever part of the device these fill
+// Clusters of 1, 2, 4, 8 and 16 blocks that a device holds at once, per thousand SMs: blocks of kWarps (whose SMs hold several), and of
+// kWideWarps.  GPCs differ in their SMs, so it is not a matter of division (148 SMs: 592, 296, 142, 71 and 31; 148, 74, 33, 15 and 7).
+constexpr int kHeld[2][5] = {{4000, 2000, 959, 479, 209}, {1000, 500, 222, 101, 47}};
 constexpr int kSmBytes = 228 << 10;  // shared memory of an SM
 constexpr float kBias = 7.f, kSlack = 4.f;   // P is kept in [0, 2^(kBias + 2 kSlack)]
 constexpr float kNone = -1e30f;      // maximum of nothing
@@ -69,6 +72,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same on a sum of zero, which then takes no registers before.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
@@ -218,8 +227,8 @@ __device__ __forceinline__ uint32_t chunk_at(int token, int chunk) {
   return uint32_t(token * 32 * GROUPS + ((chunk ^ (GROUPS == 4 ? token & 7 : (token >> 1) & 3)) << 4));
 }
 
-template <typename T, int GROUPS, int WARPS, bool LINE>
-__global__ void __launch_bounds__(WARPS * 32, WARPS == kWarps ? kBlocksPerSm : 1)
+template <typename T, int GROUPS, int WARPS, int PER_SM, bool LINE>
+__global__ void __launch_bounds__(WARPS * 32, PER_SM)
 attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ CUtensorMap map) {
   using S = Shared<GROUPS, WARPS>;
   constexpr int kDim = 32 * GROUPS, kThreads = WARPS * 32;
@@ -255,7 +264,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   int seq, offset = 0;                     // LINE: `offset` in the units of sequence `seq`, `remaining` of its share of the line, `position` on it
   int64_t remaining = 1, share = 1, position = 0;
   int head_unit = 0, rank = 0;
-  bool whole = !LINE;                      // whole units, every gridDim.x-th from this block's on
+  bool whole = !LINE;                      // whole units, `remaining` of them from `position` on
   if constexpr (LINE) {
     __shared__ int64_t sums_of[WARPS];
     __shared__ int found[2], largest_of[WARPS];
@@ -280,11 +289,13 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     largest += kUnitCost;
     share = max(int64_t(kLeastShare), (s.all + gridDim.x - 1) / gridDim.x);
     const int64_t units = int64_t(p.call.seqs) * p.head_units;
-    whole = units * largest * 4 <= s.all * 5;
+    // No unit is split where none is much longer than the others and their number fits that of the blocks.
+    const int64_t rounds = (units + gridDim.x - 1) / gridDim.x;
+    whole = units * largest * 4 <= s.all * 5 && (units >= gridDim.x ? units * 5 >= rounds * gridDim.x * 4 : units * 3 >= gridDim.x);
     if (whole) {
-      // None much longer than the others: no unit is split.
-      if (blockIdx.x >= units) return;
-      remaining = units - blockIdx.x;   // units
+      position = (blockIdx.x * units + gridDim.x - 1) / gridDim.x;   // units position ..., so that blocks with one more are spread over the SMs
+      remaining = ((blockIdx.x + 1) * units + gridDim.x - 1) / gridDim.x - position;
+      if (remaining <= 0) return;
     } else {
       position = blockIdx.x * share;
       remaining = min(share, s.all - position);
@@ -308,8 +319,10 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       offset = found[1];
     }
   }
-  int unit = LINE ? blockIdx.x : blockIdx.x / p.split;
-  if constexpr (!LINE) rank = blockIdx.x - unit * p.split;
+  if constexpr (!LINE) {
+    position = blockIdx.x / p.split;
+    rank = blockIdx.x - int(position) * p.split;
+  }
 
   const int record_rows = p.cache.page_size * 2 + p.cache.page_size / 16;
   auto place_of = [&](int t) { return int(p.page_tiles == 1 ? uint32_t(t) : __umulhi(uint32_t(t), p.by_page_tiles)); };
@@ -323,8 +336,8 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   const uint32_t odd_at = GROUPS == 4 ? chunk_at<4>(odd_token, r) : chunk_at<2>(odd_token, r >> 1) + 8 * (r & 1);
   while (remaining > 0) {
     if (whole) {
-      seq = unit / p.head_units;
-      head_unit = unit - seq * p.head_units;
+      seq = int(position) / p.head_units;
+      head_unit = int(position) - seq * p.head_units;
     }
     const Span span = span_of(p, seq);
     int begin, end, from = 0, to = 0, cost = 0;   // tiles; the part of the unit's cost
@@ -432,7 +445,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       const uint32_t scales = all_scales + slot * S::kScales + uint32_t(my_token) * (2 * GROUPS);
       // Entries outside the span may hold anything: no score, no value and no scale of theirs is used.
       const int first_position = t * kTile, length = there[warp][stage] ? span.length : 0;
-      const bool whole = first_position >= span.first && first_position + kTile <= length;
+      const bool whole_tile = first_position >= span.first && first_position + kTile <= length;
       uint32_t k[2][2 * GROUPS], ks[2], vs[2];               // tokens my_token and my_token + 8
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -450,7 +463,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
         }
       }
       bool seen[2] = {true, true};
-      if (!whole) {
+      if (!whole_tile) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int at_position = first_position + my_token + 8 * i;
@@ -459,22 +472,26 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
         }
       }
       // Scores: tokens my_token and my_token + 8, heads 2c and 2c + 1.
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      float2 sum[2];
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        float part[4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int i = GROUPS * j + g;
-          mma_f16(part, e4m3x2_to_half2(uint16_t(k[0][i])), e4m3x2_to_half2(uint16_t(k[1][i])),
-                  e4m3x2_to_half2(uint16_t(k[0][i] >> 16)), e4m3x2_to_half2(uint16_t(k[1][i] >> 16)), q[g][j][0], q[g][j][1]);
+          const uint32_t a[4] = {e4m3x2_to_half2(uint16_t(k[0][i])), e4m3x2_to_half2(uint16_t(k[1][i])),
+                                 e4m3x2_to_half2(uint16_t(k[0][i] >> 16)), e4m3x2_to_half2(uint16_t(k[1][i] >> 16))};
+          if (j == 0) mma_f16_first(part, a[0], a[1], a[2], a[3], q[g][j][0], q[g][j][1]);
+          else mma_f16(part, a[0], a[1], a[2], a[3], q[g][j][0], q[g][j][1]);
         }
-        const float low = scale_of(ks[0], g), high = scale_of(ks[1], g);
-        s[0] += low * part[0];
-        s[1] += low * part[1];
-        s[2] += high * part[2];
-        s[3] += high * part[3];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float by = scale_of(ks[i], g);
+          const float2 by2 = make_float2(by, by), part2 = make_float2(part[2 * i], part[2 * i + 1]);
+          sum[i] = g == 0 ? mul2(by2, part2) : fma2(by2, part2, sum[i]);
+        }
       }
+      const float s[4] = {sum[0].x, sum[0].y, sum[1].x, sum[1].y};
       uint32_t v[4][GROUPS];                                 // tokens value_token, odd_token and those eight behind: elements 32 g + 4 r ...
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -490,7 +507,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       // The tile before this one has been multiplied by all lanes; its stage takes the next copy.
       __syncwarp();
       copy_next();
-      if (!whole) {
+      if (!whole_tile) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int at_position = first_position + (i & 1 ? odd_token : value_token) + 8 * (i >> 1);
@@ -502,7 +519,12 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       }
       float x[4], scale[2][GROUPS], top = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = seen[i >> 1] ? s[i] * to_log2[i & 1] + shift[i & 1] : -INFINITY;
+      for (int i = 0; i < 4; ++i) x[i] = s[i] * to_log2[i & 1] + shift[i & 1];
+      if (!whole_tile) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!seen[i >> 1]) x[i] = -INFINITY;
+      }
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
@@ -535,21 +557,25 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
           }
         }
       }
-      float probability[4];
+      float2 probability[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) probability[i] = exp2_approx(x[i]);
-      weight[0] += probability[0] + probability[2];
-      weight[1] += probability[1] + probability[3];
+      for (int i = 0; i < 2; ++i) probability[i] = make_float2(exp2_approx(x[2 * i]), exp2_approx(x[2 * i + 1]));
+      weight[0] += probability[0].x + probability[1].x;
+      weight[1] += probability[0].y + probability[1].y;
 
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
-        const uint32_t b0 = transpose8x8(half2_bits(probability[0] * scale[0][g], probability[1] * scale[0][g]));
-        const uint32_t b1 = transpose8x8(half2_bits(probability[2] * scale[1][g], probability[3] * scale[1][g]));
+        uint32_t b[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 scaled = mul2(probability[i], make_float2(scale[i][g], scale[i][g]));
+          b[i] = transpose8x8(half2_bits(scaled.x, scaled.y));
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t near = __byte_perm(v[0][g], v[1][g], h ? 0x7362 : 0x5140), far = __byte_perm(v[2][g], v[3][g], h ? 0x7362 : 0x5140);
           mma_f16(out[g][h], e4m3x2_to_half2(uint16_t(near)), e4m3x2_to_half2(uint16_t(near >> 16)),
-                  e4m3x2_to_half2(uint16_t(far)), e4m3x2_to_half2(uint16_t(far >> 16)), b0, b1);
+                  e4m3x2_to_half2(uint16_t(far)), e4m3x2_to_half2(uint16_t(far >> 16)), b[0], b[1]);
         }
       }
       if (stage == ring - 1) {
@@ -630,8 +656,8 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
         for (int i = threadIdx.x; i < others; i += kThreads) p.tags[blockIdx.x + 1 + i] = 0;
       }
       if (whole) {
-        remaining -= gridDim.x;
-        unit += gridDim.x;
+        --remaining;
+        ++position;
       } else {
         remaining -= to - from;
         offset += to - from;
@@ -672,9 +698,10 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   }
 }
 
-// How a call is spread over the device: blocks with an SM each in clusters of `split`, or a line (or whole units where sequences are short).
-struct Split { int chunks, head_units, split; int64_t units; bool wide, line; int blocks, ring; };
-Split split_of(const hg_cache& c, int seqs, int heads, int table_width, int window) {
+// How a call is spread over the device.
+struct Split { int chunks, head_units; int64_t units; int warps, per_sm, split; bool line; int blocks, ring; };
+
+int sm_count() {
   static const int sms = [] {
     int device = 0, n = 148;
     if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
@@ -683,22 +710,43 @@ Split split_of(const hg_cache& c, int seqs, int heads, int table_width, int wind
     }
     return n;
   }();
-  Split s;
-  const int group = heads / c.kv_heads;
+  return sms;
+}
+
+Split split_of(const hg_cache& c, int seqs, int heads, int table_width, int window) {
+  Split s{};
+  const int group = heads / c.kv_heads, sms = sm_count();
   s.chunks = (group + kHeadTile - 1) / kHeadTile;
   s.head_units = c.kv_heads * s.chunks;
   s.units = int64_t(seqs) * s.head_units;
   int64_t longest = (int64_t(table_width) * c.page_size + kTile - 1) / kTile;
   if (window) longest = std::min<int64_t>(longest, (int64_t(window) + 2 * kTile - 2) / kTile);
-  s.wide = s.units <= sms && longest > kWhole;
-  s.line = !s.wide && longest > kWhole;
+  s.warps = kWarps;
+  s.per_sm = kBlocksPerSm;
   s.split = 1;
-  while (s.wide && s.split < kMostSplit && s.units * s.split * 2 <= sms && longest > s.split * kWideWarps) s.split *= 2;
-  s.blocks = int(s.line ? std::min<int64_t>(sms * kBlocksPerSm, (s.units * (longest + kUnitCost) + kLeastShare - 1) / kLeastShare) : s.units * s.split);
+  // The most warps of which the device holds all clusters at once.
+  int64_t most = longest > kWhole ? 0 : INT64_MAX;
+  for (int wide = 0; wide < 2; ++wide)
+    for (int log = 0; log < 5; ++log) {
+      const int warps = wide ? kWideWarps : kWarps, split = 1 << log;
+      const int64_t all = s.units * split * warps;
+      if (s.units * 1000 > int64_t(sms) * kHeld[wide][log] || all <= most || (split > 1 && longest <= int64_t(split / 2) * warps)) continue;
+      most = all;
+      s.warps = warps;
+      s.per_sm = wide ? 1 : kBlocksPerSm;
+      s.split = split;
+    }
+  s.line = longest > kWhole && (s.units > sms || (s.units * longest > kFew && most * 4 < int64_t(sms) * kWideWarps * 3));
+  s.blocks = int(s.units * s.split);
+  if (s.line) {
+    s.warps = kWarps;
+    s.per_sm = s.units <= sms * kLineBlocksPerSm ? kLineBlocksPerSm : kBlocksPerSm;
+    s.split = 1;
+    s.blocks = int(std::min<int64_t>(sms * s.per_sm, (s.units * (longest + kUnitCost) + kLeastShare - 1) / kLeastShare));
+  }
   // As deep a ring as the blocks of an SM have room for, and use.
-  const int per_sm = s.wide ? 1 : kBlocksPerSm, warps = s.wide ? kWideWarps : kWarps;
-  const int room = (kSmBytes / per_sm - 2048) / (warps * (c.head_dim == 128 ? Shared<4, kWarps>::kStage : Shared<2, kWarps>::kStage));
-  s.ring = std::max(2, std::min({kMostRing, room, int((longest / s.split + warps - 1) / warps) + 1}));
+  const int room = (kSmBytes / s.per_sm - 2048) / (s.warps * (c.head_dim == 128 ? Shared<4, kWarps>::kStage : Shared<2, kWarps>::kStage));
+  s.ring = std::max(2, std::min({kMostRing, room, int((longest / s.split + s.warps - 1) / s.warps) + 1}));
   return s;
 }
 
@@ -727,7 +775,7 @@ CUtensorMap cache_map(const hg_cache& c) {
   return map;
 }
 
-template <typename T, int GROUPS, int WARPS, bool LINE>
+template <typename T, int GROUPS, int WARPS, int PER_SM, bool LINE>
 void launch_attention(const AttentionParams& p, const Split& s, cudaStream_t stream) {
   const int bytes = Shared<GROUPS, WARPS>::bytes(s.ring);
   static std::once_flag once[64];   // limits of the function on each device
@@ -735,8 +783,8 @@ void launch_attention(const AttentionParams& p, const Split& s, cudaStream_t str
   check(cudaGetDevice(&device), "cudaGetDevice");
   if (device < 0 || device >= 64) throw std::runtime_error("Device ordinals 0..63 are supported");
   std::call_once(once[device], [] {
-    check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, WARPS, LINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shared<GROUPS, WARPS>::bytes(kMostRing)), "attention");
-    check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, WARPS, LINE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "attention");
+    check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, WARPS, PER_SM, LINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shared<GROUPS, WARPS>::bytes(kMostRing)), "attention");
+    check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, WARPS, PER_SM, LINE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "attention");
   });
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(unsigned(s.blocks));
@@ -755,7 +803,7 @@ void launch_attention(const AttentionParams& p, const Split& s, cudaStream_t str
   }
   config.attrs = attribute;
   config.numAttrs = unsigned(count);
-  check(cudaLaunchKernelEx(&config, attention_kernel<T, GROUPS, WARPS, LINE>, p, cache_map(p.cache)), "attention");
+  check(cudaLaunchKernelEx(&config, attention_kernel<T, GROUPS, WARPS, PER_SM, LINE>, p, cache_map(p.cache)), "attention");
 }
 
 }  // namespace
@@ -801,7 +849,9 @@ int hg_attention(const hg_cache* cache, const hg_attention_call* call, int dtype
   const auto pick = [&](auto type, auto groups) {
     using T = decltype(type);
     constexpr int G = decltype(groups)::value;
-    return s.wide ? hg::launch_attention<T, G, hg::kWideWarps, false> : s.line ? hg::launch_attention<T, G, hg::kWarps, true> : hg::launch_attention<T, G, hg::kWarps, false>;
+    if (s.line)
+      return s.per_sm == hg::kLineBlocksPerSm ? hg::launch_attention<T, G, hg::kWarps, hg::kLineBlocksPerSm, true> : hg::launch_attention<T, G, hg::kWarps, hg::kBlocksPerSm, true>;
+    return s.warps == hg::kWideWarps ? hg::launch_attention<T, G, hg::kWideWarps, 1, false> : hg::launch_attention<T, G, hg::kWarps, hg::kBlocksPerSm, false>;
   };
   using Two = std::integral_constant<int, 2>;
   using Four = std::integral_constant<int, 4>;
