@@ -1,7 +1,7 @@
 // A paged key-value cache held in MXFP8: quantising keys and values as they are written, and reading entries back.
 //
 // E4M3 codes with an E8M0 scale per 32 elements of a head, by the rule of hg_pack.  The layout is the one that
-// hg_attention.cu's loads ask for (see hg_cache_layout in hg_cache.cuh).
+// hg_attention.cu's loads ask for (see hg_cache.cuh).  Both are bound by memory, and in small calls by their chain: slot, entry.
 #include <algorithm>
 
 #include "hg_cache.cuh"
@@ -9,108 +9,117 @@
 namespace hg {
 namespace {
 
-// Eight threads to a token, head and key or value; each has four elements of every group of 32, its 4 x GROUPS codes are consecutive in the cache.
+// Eight threads to a token, head and key or value; each has four elements of every group of 32, whose 4 x GROUPS codes are consecutive in
+// the cache.  A block has kTokens tokens of one head.
+constexpr int kTokens = 8, kThreads = kTokens * 16;
+struct Place { uint8_t *codes, *scales; };   // of one thread's part of an entry
+template <int GROUPS>
+__device__ __forceinline__ Place place_of(const hg_cache& c, uint64_t by_page_size, uint32_t slot, int head, int kind, int x) {
+  const uint32_t page = uint32_t(__umul64hi(slot, by_page_size)), at = slot - page * uint32_t(c.page_size);
+  uint8_t* const record = static_cast<uint8_t*>(c.data) + (int64_t(page) * c.kv_heads + head) * cache_page_bytes(c.page_size, 32 * GROUPS);
+  return {record + (kind * c.page_size + int(at)) * (32 * GROUPS) + x * (4 * GROUPS), record + 2 * c.page_size * (32 * GROUPS) + (2 * int(at) + kind) * GROUPS};
+}
+
 template <typename T, int GROUPS>
-__global__ void __launch_bounds__(256)
-cache_write_kernel(const hg_cache c, const uint16_t* k, const uint16_t* v, int64_t k_token, int64_t k_head,
+__global__ void __launch_bounds__(kThreads)
+cache_write_kernel(const hg_cache c, uint64_t by_page_size, const uint16_t* k, const uint16_t* v, int64_t k_token, int64_t k_head,
                    int64_t v_token, int64_t v_head, const int64_t* slots, int tokens) {
   pdl_trigger();
-  const int64_t thread = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int x = int(thread & 7);
-  const int64_t row = thread >> 3;                       // token, head, key or value
-  const int kind = int(row & 1);
-  const int64_t pair = row >> 1;
-  const int64_t token = pair / c.kv_heads;
-  const int head = int(pair - token * c.kv_heads);
-  pdl_wait();
+  const int x = threadIdx.x & 7, kind = (threadIdx.x >> 3) & 1, head = blockIdx.y;
+  const int64_t token = int64_t(blockIdx.x) * kTokens + (threadIdx.x >> 4);
   if (token >= tokens) return;                           // whole groups of eight
-  const int64_t slot = slots[token];
-  if (slot < 0 || slot >= int64_t(c.pages) * c.page_size) return;
-  const unsigned mask = 0xffu << (threadIdx.x & 24);
   const uint16_t* const src = (kind ? v + token * v_token + head * v_head : k + token * k_token + head * k_head) + 4 * x;
+  pdl_wait();
+  const int64_t slot = slots[token];
   uint2 raw[GROUPS];
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) raw[g] = *reinterpret_cast<const uint2*>(src + 32 * g);
-  const int64_t page = slot / c.page_size;
-  const int at = int(slot - page * c.page_size);
-  uint8_t* const record = static_cast<uint8_t*>(c.data) + (page * c.kv_heads + head) * cache_page_bytes(c.page_size, 32 * GROUPS);
+  if (uint64_t(slot) >= uint64_t(c.pages) * uint64_t(c.page_size)) return;
+  const Place to = place_of<GROUPS>(c, by_page_size, uint32_t(slot), head, kind, x);
+  const unsigned mask = 0xffu << (threadIdx.x & 24);
   uint32_t codes[GROUPS], scales = 0;
+  // The largest of two groups at once, as pairs of 16-bit values; a NaN is skipped.
+  float top[GROUPS];
+#pragma unroll
+  for (int g = 0; g < GROUPS; g += 2) {
+    uint32_t a = Packed<T>::max_abs(Packed<T>::max_abs(0u, raw[g].x), raw[g].y), b = Packed<T>::max_abs(Packed<T>::max_abs(0u, raw[g + 1].x), raw[g + 1].y);
+    uint32_t both = Packed<T>::max_abs(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+#pragma unroll
+    for (int step = 1; step < 8; step <<= 1) both = Packed<T>::max_abs(both, __shfl_xor_sync(mask, both, step));
+    const float2 ends = Packed<T>::widen(both);
+    top[g] = fmaxf(0.f, ends.x);
+    top[g + 1] = fmaxf(0.f, ends.y);
+  }
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
-    const float2 low = Packed<T>::widen(raw[g].x), high = Packed<T>::widen(raw[g].y);
-    float amax = fmaxf(fmaxf(fmaxf(0.f, fabsf(low.x)), fabsf(low.y)), fmaxf(fabsf(high.x), fabsf(high.y)));
-#pragma unroll
-    for (int step = 1; step < 8; step <<= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, step));
-    const int e = mx_exponent<false>(amax);
+    const int e = mx_exponent<false>(top[g]);
     const float inv = mx_inverse_scale(e);
-    codes[g] = cvt_e4m3x2(low.x * inv, low.y * inv) | (cvt_e4m3x2(high.x * inv, high.y * inv) << 16);
+    const float2 low = mul2(Packed<T>::widen(raw[g].x), make_float2(inv, inv)), high = mul2(Packed<T>::widen(raw[g].y), make_float2(inv, inv));
+    codes[g] = cvt_e4m3x2(low.x, low.y) | (cvt_e4m3x2(high.x, high.y) << 16);
     scales |= uint32_t(e + 127) << (8 * g);
   }
-  uint8_t* const to = record + (int64_t(kind) * c.page_size + at) * (32 * GROUPS) + x * (4 * GROUPS);
-  if constexpr (GROUPS == 4) *reinterpret_cast<uint4*>(to) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-  else *reinterpret_cast<uint2*>(to) = make_uint2(codes[0], codes[1]);
-  uint8_t* const scale = record + int64_t(2) * c.page_size * (32 * GROUPS) + (2 * at + kind) * GROUPS;
+  if constexpr (GROUPS == 4) *reinterpret_cast<uint4*>(to.codes) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+  else *reinterpret_cast<uint2*>(to.codes) = make_uint2(codes[0], codes[1]);
   if (x == 0) {
-    if constexpr (GROUPS == 4) *reinterpret_cast<uint32_t*>(scale) = scales;
-    else *reinterpret_cast<uint16_t*>(scale) = uint16_t(scales);
+    if constexpr (GROUPS == 4) *reinterpret_cast<uint32_t*>(to.scales) = scales;
+    else *reinterpret_cast<uint16_t*>(to.scales) = uint16_t(scales);
   }
 }
 
 template <typename T, int GROUPS>
-__global__ void __launch_bounds__(256)
-cache_read_kernel(const hg_cache c, uint16_t* k, uint16_t* v, const int64_t* slots, int tokens) {
+__global__ void __launch_bounds__(kThreads)
+cache_read_kernel(const hg_cache c, uint64_t by_page_size, uint16_t* k, uint16_t* v, const int64_t* slots, int tokens) {
   pdl_trigger();
-  const int64_t thread = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int x = int(thread & 7);
-  const int64_t row = thread >> 3;
-  const int kind = int(row & 1);
-  const int64_t pair = row >> 1;
-  const int64_t token = pair / c.kv_heads;
-  const int head = int(pair - token * c.kv_heads);
-  pdl_wait();
+  const int x = threadIdx.x & 7, kind = (threadIdx.x >> 3) & 1, head = blockIdx.y;
+  const int64_t token = int64_t(blockIdx.x) * kTokens + (threadIdx.x >> 4);
   if (token >= tokens) return;
+  uint16_t* const to = (kind ? v : k) + (token * c.kv_heads + head) * (32 * GROUPS) + 4 * x;
+  pdl_wait();
   const int64_t slot = slots[token];
   uint32_t codes[GROUPS] = {}, scales = 0;
-  if (slot >= 0 && slot < int64_t(c.pages) * c.page_size) {
-    const int64_t page = slot / c.page_size;
-    const int at = int(slot - page * c.page_size);
-    const uint8_t* const record = static_cast<const uint8_t*>(c.data) + (page * c.kv_heads + head) * cache_page_bytes(c.page_size, 32 * GROUPS);
-    const uint8_t* const from = record + (int64_t(kind) * c.page_size + at) * (32 * GROUPS) + x * (4 * GROUPS);
-    const uint8_t* const scale = record + int64_t(2) * c.page_size * (32 * GROUPS) + (2 * at + kind) * GROUPS;
+  if (uint64_t(slot) < uint64_t(c.pages) * uint64_t(c.page_size)) {
+    const Place from = place_of<GROUPS>(c, by_page_size, uint32_t(slot), head, kind, x);
     if constexpr (GROUPS == 4) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(from);
+      const uint4 raw = *reinterpret_cast<const uint4*>(from.codes);
       codes[0] = raw.x; codes[1] = raw.y; codes[2] = raw.z; codes[3] = raw.w;
-      scales = *reinterpret_cast<const uint32_t*>(scale);
+      scales = *reinterpret_cast<const uint32_t*>(from.scales);
     } else {
-      const uint2 raw = *reinterpret_cast<const uint2*>(from);
+      const uint2 raw = *reinterpret_cast<const uint2*>(from.codes);
       codes[0] = raw.x; codes[1] = raw.y;
-      scales = *reinterpret_cast<const uint16_t*>(scale);
+      scales = *reinterpret_cast<const uint16_t*>(from.scales);
     }
   }
-  uint16_t* const to = (kind ? v : k) + pair * (32 * GROUPS) + 4 * x;
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
     const float scale = mx_scale(int(scales >> (8 * g)) & 255);
-    const float2 low = e4m3x2_to_float2(uint16_t(codes[g])), high = e4m3x2_to_float2(uint16_t(codes[g] >> 16));
-    *reinterpret_cast<uint2*>(to + 32 * g) = make_uint2(
-        uint32_t(from_float<T>(low.x * scale)) | (uint32_t(from_float<T>(low.y * scale)) << 16),
-        uint32_t(from_float<T>(high.x * scale)) | (uint32_t(from_float<T>(high.y * scale)) << 16));
+    const float2 low = mul2(e4m3x2_to_float2(uint16_t(codes[g])), make_float2(scale, scale)), high = mul2(e4m3x2_to_float2(uint16_t(codes[g] >> 16)), make_float2(scale, scale));
+    *reinterpret_cast<uint2*>(to + 32 * g) = make_uint2(Packed<T>::round(low), Packed<T>::round(high));
   }
 }
 
-unsigned row_blocks(const hg_cache& c, int tokens) {
-  const int64_t blocks = (int64_t(tokens) * c.kv_heads * 16 + 255) / 256;
-  if (blocks > 0x7fffffff) throw std::runtime_error("hg_cache: too many tokens in one call");
-  return unsigned(blocks);
-}
+dim3 token_blocks(const hg_cache& c, int tokens) { return dim3(unsigned((tokens + kTokens - 1) / kTokens), unsigned(c.kv_heads)); }
+uint64_t inverse_of(int n) { return ~uint64_t(0) / uint64_t(n) + 1; }   // ceil(2^64 / n) for n > 1; exact for 32-bit dividends
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
+
+int sm_count() {
+  static const int sms = [] {
+    int device = 0, n = 148;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+      cudaGetLastError();
+      n = 148;
+    }
+    return n;
+  }();
+  return sms;
+}
 
 void validate_cache(const hg_cache& c) {
   if (!c.data || c.pages <= 0 || c.kv_heads <= 0) throw std::runtime_error("hg_cache: a cache has pages and heads");
   if (c.head_dim != 64 && c.head_dim != 128) throw std::runtime_error("hg_cache: head_dim must be 64 or 128");
   if (c.page_size <= 0 || c.page_size % 16 || c.page_size > 1024) throw std::runtime_error("hg_cache: page_size must be a multiple of 16 up to 1024");
+  if (c.kv_heads > 65535 || int64_t(c.pages) * c.page_size > 0x7fffffff) throw std::runtime_error("hg_cache: too many heads or entries");
   if (!aligned16(c.data)) throw std::runtime_error("hg_cache: data must be aligned to 16 bytes");
 }
 
@@ -136,7 +145,7 @@ int hg_cache_write(const hg_cache* cache, const void* k, const void* v, const in
   const bool bf16 = dtype == HG_DTYPE_BF16, wide = cache->head_dim == 128;
   const auto kernel = bf16 ? (wide ? hg::cache_write_kernel<__nv_bfloat16, 4> : hg::cache_write_kernel<__nv_bfloat16, 2>)
                            : (wide ? hg::cache_write_kernel<__half, 4> : hg::cache_write_kernel<__half, 2>);
-  hg::check(hg::launch_kernel(kernel, dim3(hg::row_blocks(*cache, tokens)), dim3(256), 0, static_cast<cudaStream_t>(stream), *cache, kk, vv,
+  hg::check(hg::launch_kernel(kernel, hg::token_blocks(*cache, tokens), dim3(hg::kThreads), 0, static_cast<cudaStream_t>(stream), *cache, hg::inverse_of(cache->page_size), kk, vv,
                               strides[0], strides[1], strides[2], strides[3], slots, tokens), "cache write");
   HG_CATCH
 }
@@ -152,7 +161,7 @@ int hg_cache_read(const hg_cache* cache, void* k, void* v, const int64_t* slots,
   const bool bf16 = dtype == HG_DTYPE_BF16, wide = cache->head_dim == 128;
   const auto kernel = bf16 ? (wide ? hg::cache_read_kernel<__nv_bfloat16, 4> : hg::cache_read_kernel<__nv_bfloat16, 2>)
                            : (wide ? hg::cache_read_kernel<__half, 4> : hg::cache_read_kernel<__half, 2>);
-  hg::check(hg::launch_kernel(kernel, dim3(hg::row_blocks(*cache, tokens)), dim3(256), 0, static_cast<cudaStream_t>(stream), *cache,
+  hg::check(hg::launch_kernel(kernel, hg::token_blocks(*cache, tokens), dim3(hg::kThreads), 0, static_cast<cudaStream_t>(stream), *cache, hg::inverse_of(cache->page_size),
                               static_cast<uint16_t*>(k), static_cast<uint16_t*>(v), slots, tokens), "cache read");
   HG_CATCH
 }

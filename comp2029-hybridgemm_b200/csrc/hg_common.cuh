@@ -70,6 +70,7 @@ __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.lau
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 bool pdl_enabled();
+int sm_count();   // of the first device that asks; devices of one machine are alike
 
 template <typename... KernelArgs, typename... Args>
 inline cudaError_t launch_kernel(void (*kernel)(KernelArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
@@ -155,6 +156,7 @@ template <> struct Packed<__half> {
     return *reinterpret_cast<const uint32_t*>(&m);
   }
   static __device__ __forceinline__ float2 widen(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+  static __device__ __forceinline__ uint32_t round(float2 v) { const __half2 h = __floats2half2_rn(v.x, v.y); return *reinterpret_cast<const uint32_t*>(&h); }
   static __device__ __forceinline__ uint32_t swiglu(float2 act, uint32_t up) {   // (up + 0) as in silu8
     const __half2 p = __hmul2(__floats2half2_rn(act.x, act.y), __hadd2(*reinterpret_cast<const __half2*>(&up), __float2half2_rn(0.f)));
     return *reinterpret_cast<const uint32_t*>(&p);
@@ -170,6 +172,7 @@ template <> struct Packed<__nv_bfloat16> {
     return *reinterpret_cast<const uint32_t*>(&m);
   }
   static __device__ __forceinline__ float2 widen(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+  static __device__ __forceinline__ uint32_t round(float2 v) { const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y); return *reinterpret_cast<const uint32_t*>(&h); }
   static __device__ __forceinline__ uint32_t swiglu(float2 act, uint32_t up) {
     const __nv_bfloat162 p = __hmul2(__floats2bfloat162_rn(act.x, act.y), __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&up), __float2bfloat162_rn(0.f)));
     return *reinterpret_cast<const uint32_t*>(&p);
