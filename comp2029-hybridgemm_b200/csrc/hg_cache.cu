@@ -2,7 +2,7 @@
 //
 // E4M3 codes with an E8M0 scale per 32 elements of a head, by the rule of hg_pack.  The layout is the one that
 // hg_attention.cu's loads ask for (see hg_cache.cuh).  Both are bound by memory, and in small calls by their chain: slot, entry.
-#include <algorithm>
+#include <type_traits>
 
 #include "hg_cache.cuh"
 
@@ -12,6 +12,7 @@ namespace {
 // Eight threads to a token, head and key or value; each has four elements of every group of 32, whose 4 x GROUPS codes are consecutive in
 // the cache.  A block has kTokens tokens of one head.
 constexpr int kTokens = 8, kThreads = kTokens * 16;
+constexpr int kMany = 32768;   // tokens times heads from which a thread has two tokens
 struct Place { uint8_t *codes, *scales; };   // of one thread's part of an entry
 template <int GROUPS>
 __device__ __forceinline__ Place place_of(const hg_cache& c, uint64_t by_page_size, uint32_t slot, int head, int kind, int x) {
@@ -20,84 +21,105 @@ __device__ __forceinline__ Place place_of(const hg_cache& c, uint64_t by_page_si
   return {record + (kind * c.page_size + int(at)) * (32 * GROUPS) + x * (4 * GROUPS), record + 2 * c.page_size * (32 * GROUPS) + (2 * int(at) + kind) * GROUPS};
 }
 
-template <typename T, int GROUPS>
+// EACH tokens to a thread, their loads under way together.
+template <typename T, int GROUPS, int EACH>
 __global__ void __launch_bounds__(kThreads)
 cache_write_kernel(const hg_cache c, uint64_t by_page_size, const uint16_t* k, const uint16_t* v, int64_t k_token, int64_t k_head,
                    int64_t v_token, int64_t v_head, const int64_t* slots, int tokens) {
   pdl_trigger();
   const int x = threadIdx.x & 7, kind = (threadIdx.x >> 3) & 1, head = blockIdx.y;
-  const int64_t token = int64_t(blockIdx.x) * kTokens + (threadIdx.x >> 4);
-  if (token >= tokens) return;                           // whole groups of eight
-  const uint16_t* const src = (kind ? v + token * v_token + head * v_head : k + token * k_token + head * k_head) + 4 * x;
-  pdl_wait();
-  const int64_t slot = slots[token];
-  uint2 raw[GROUPS];
-#pragma unroll
-  for (int g = 0; g < GROUPS; ++g) raw[g] = *reinterpret_cast<const uint2*>(src + 32 * g);
-  if (uint64_t(slot) >= uint64_t(c.pages) * uint64_t(c.page_size)) return;
-  const Place to = place_of<GROUPS>(c, by_page_size, uint32_t(slot), head, kind, x);
+  const int64_t first = int64_t(blockIdx.x) * (kTokens * EACH) + (threadIdx.x >> 4), stride = kind ? v_token : k_token;
+  const uint16_t* const src = (kind ? v + head * v_head : k + head * k_head) + 4 * x;
   const unsigned mask = 0xffu << (threadIdx.x & 24);
-  uint32_t codes[GROUPS], scales = 0;
-  // The largest of two groups at once, as pairs of 16-bit values; a NaN is skipped.
-  float top[GROUPS];
+  if (first >= tokens) return;
+  pdl_wait();
+  int64_t slot[EACH];
+  uint2 raw[EACH][GROUPS];
 #pragma unroll
-  for (int g = 0; g < GROUPS; g += 2) {
-    uint32_t a = Packed<T>::max_abs(Packed<T>::max_abs(0u, raw[g].x), raw[g].y), b = Packed<T>::max_abs(Packed<T>::max_abs(0u, raw[g + 1].x), raw[g + 1].y);
-    uint32_t both = Packed<T>::max_abs(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+  for (int i = 0; i < EACH; ++i) {
+    slot[i] = -1;
+    if (i && first + i * kTokens >= tokens) continue;   // whole groups of eight
+    slot[i] = slots[first + i * kTokens];
 #pragma unroll
-    for (int step = 1; step < 8; step <<= 1) both = Packed<T>::max_abs(both, __shfl_xor_sync(mask, both, step));
-    const float2 ends = Packed<T>::widen(both);
-    top[g] = fmaxf(0.f, ends.x);
-    top[g + 1] = fmaxf(0.f, ends.y);
+    for (int g = 0; g < GROUPS; ++g) raw[i][g] = *reinterpret_cast<const uint2*>(src + (first + i * kTokens) * stride + 32 * g);
   }
 #pragma unroll
-  for (int g = 0; g < GROUPS; ++g) {
-    const int e = mx_exponent<false>(top[g]);
-    const float inv = mx_inverse_scale(e);
-    const float2 low = mul2(Packed<T>::widen(raw[g].x), make_float2(inv, inv)), high = mul2(Packed<T>::widen(raw[g].y), make_float2(inv, inv));
-    codes[g] = cvt_e4m3x2(low.x, low.y) | (cvt_e4m3x2(high.x, high.y) << 16);
-    scales |= uint32_t(e + 127) << (8 * g);
-  }
-  if constexpr (GROUPS == 4) *reinterpret_cast<uint4*>(to.codes) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-  else *reinterpret_cast<uint2*>(to.codes) = make_uint2(codes[0], codes[1]);
-  if (x == 0) {
-    if constexpr (GROUPS == 4) *reinterpret_cast<uint32_t*>(to.scales) = scales;
-    else *reinterpret_cast<uint16_t*>(to.scales) = uint16_t(scales);
+  for (int i = 0; i < EACH; ++i) {
+    if (uint64_t(slot[i]) >= uint64_t(c.pages) * uint64_t(c.page_size)) continue;
+    const Place to = place_of<GROUPS>(c, by_page_size, uint32_t(slot[i]), head, kind, x);
+    uint32_t codes[GROUPS], scales = 0;
+    // The largest of two groups at once, as pairs of 16-bit values; a NaN is skipped.
+    float top[GROUPS];
+#pragma unroll
+    for (int g = 0; g < GROUPS; g += 2) {
+      const uint32_t a = Packed<T>::max_abs(Packed<T>::max_abs(0u, raw[i][g].x), raw[i][g].y), b = Packed<T>::max_abs(Packed<T>::max_abs(0u, raw[i][g + 1].x), raw[i][g + 1].y);
+      uint32_t both = Packed<T>::max_abs(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+#pragma unroll
+      for (int step = 1; step < 8; step <<= 1) both = Packed<T>::max_abs(both, __shfl_xor_sync(mask, both, step));
+      const float2 ends = Packed<T>::widen(both);
+      top[g] = fmaxf(0.f, ends.x);
+      top[g + 1] = fmaxf(0.f, ends.y);
+    }
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      const int e = mx_exponent<false>(top[g]);
+      const float inv = mx_inverse_scale(e);
+      const float2 low = mul2(Packed<T>::widen(raw[i][g].x), make_float2(inv, inv)), high = mul2(Packed<T>::widen(raw[i][g].y), make_float2(inv, inv));
+      codes[g] = cvt_e4m3x2(low.x, low.y) | (cvt_e4m3x2(high.x, high.y) << 16);
+      scales |= uint32_t(e + 127) << (8 * g);
+    }
+    if constexpr (GROUPS == 4) *reinterpret_cast<uint4*>(to.codes) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+    else *reinterpret_cast<uint2*>(to.codes) = make_uint2(codes[0], codes[1]);
+    if (x == 0) {
+      if constexpr (GROUPS == 4) *reinterpret_cast<uint32_t*>(to.scales) = scales;
+      else *reinterpret_cast<uint16_t*>(to.scales) = uint16_t(scales);
+    }
   }
 }
 
-template <typename T, int GROUPS>
+template <typename T, int GROUPS, int EACH>
 __global__ void __launch_bounds__(kThreads)
 cache_read_kernel(const hg_cache c, uint64_t by_page_size, uint16_t* k, uint16_t* v, const int64_t* slots, int tokens) {
   pdl_trigger();
   const int x = threadIdx.x & 7, kind = (threadIdx.x >> 3) & 1, head = blockIdx.y;
-  const int64_t token = int64_t(blockIdx.x) * kTokens + (threadIdx.x >> 4);
-  if (token >= tokens) return;
-  uint16_t* const to = (kind ? v : k) + (token * c.kv_heads + head) * (32 * GROUPS) + 4 * x;
+  const int64_t first = int64_t(blockIdx.x) * (kTokens * EACH) + (threadIdx.x >> 4);
+  uint16_t* const to = (kind ? v : k) + head * (32 * GROUPS) + 4 * x;
   pdl_wait();
-  const int64_t slot = slots[token];
-  uint32_t codes[GROUPS] = {}, scales = 0;
-  if (uint64_t(slot) < uint64_t(c.pages) * uint64_t(c.page_size)) {
-    const Place from = place_of<GROUPS>(c, by_page_size, uint32_t(slot), head, kind, x);
+  int64_t slot[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) slot[i] = first + i * kTokens < tokens ? slots[first + i * kTokens] : -1;
+  uint32_t codes[EACH][GROUPS], scales[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) codes[i][g] = 0;
+    scales[i] = 0;
+    if (uint64_t(slot[i]) >= uint64_t(c.pages) * uint64_t(c.page_size)) continue;
+    const Place from = place_of<GROUPS>(c, by_page_size, uint32_t(slot[i]), head, kind, x);
     if constexpr (GROUPS == 4) {
       const uint4 raw = *reinterpret_cast<const uint4*>(from.codes);
-      codes[0] = raw.x; codes[1] = raw.y; codes[2] = raw.z; codes[3] = raw.w;
-      scales = *reinterpret_cast<const uint32_t*>(from.scales);
+      codes[i][0] = raw.x; codes[i][1] = raw.y; codes[i][2] = raw.z; codes[i][3] = raw.w;
+      scales[i] = *reinterpret_cast<const uint32_t*>(from.scales);
     } else {
       const uint2 raw = *reinterpret_cast<const uint2*>(from.codes);
-      codes[0] = raw.x; codes[1] = raw.y;
-      scales = *reinterpret_cast<const uint16_t*>(from.scales);
+      codes[i][0] = raw.x; codes[i][1] = raw.y;
+      scales[i] = *reinterpret_cast<const uint16_t*>(from.scales);
     }
   }
 #pragma unroll
-  for (int g = 0; g < GROUPS; ++g) {
-    const float scale = mx_scale(int(scales >> (8 * g)) & 255);
-    const float2 low = mul2(e4m3x2_to_float2(uint16_t(codes[g])), make_float2(scale, scale)), high = mul2(e4m3x2_to_float2(uint16_t(codes[g] >> 16)), make_float2(scale, scale));
-    *reinterpret_cast<uint2*>(to + 32 * g) = make_uint2(Packed<T>::round(low), Packed<T>::round(high));
+  for (int i = 0; i < EACH; ++i) {
+    if (first + i * kTokens >= tokens) return;
+    uint16_t* const row = to + (first + i * kTokens) * c.kv_heads * (32 * GROUPS);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      const float scale = mx_scale(int(scales[i] >> (8 * g)) & 255);
+      const float2 low = mul2(e4m3x2_to_float2(uint16_t(codes[i][g])), make_float2(scale, scale)), high = mul2(e4m3x2_to_float2(uint16_t(codes[i][g] >> 16)), make_float2(scale, scale));
+      *reinterpret_cast<uint2*>(row + 32 * g) = make_uint2(Packed<T>::round(low), Packed<T>::round(high));
+    }
   }
 }
 
-dim3 token_blocks(const hg_cache& c, int tokens) { return dim3(unsigned((tokens + kTokens - 1) / kTokens), unsigned(c.kv_heads)); }
+dim3 token_blocks(const hg_cache& c, int tokens, int each) { return dim3(unsigned((tokens + kTokens * each - 1) / (kTokens * each)), unsigned(c.kv_heads)); }
 uint64_t inverse_of(int n) { return ~uint64_t(0) / uint64_t(n) + 1; }   // ceil(2^64 / n) for n > 1; exact for 32-bit dividends
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -143,9 +165,16 @@ int hg_cache_write(const hg_cache* cache, const void* k, const void* v, const in
   const auto* kk = static_cast<const uint16_t*>(k);
   const auto* vv = static_cast<const uint16_t*>(v);
   const bool bf16 = dtype == HG_DTYPE_BF16, wide = cache->head_dim == 128;
-  const auto kernel = bf16 ? (wide ? hg::cache_write_kernel<__nv_bfloat16, 4> : hg::cache_write_kernel<__nv_bfloat16, 2>)
-                           : (wide ? hg::cache_write_kernel<__half, 4> : hg::cache_write_kernel<__half, 2>);
-  hg::check(hg::launch_kernel(kernel, hg::token_blocks(*cache, tokens), dim3(hg::kThreads), 0, static_cast<cudaStream_t>(stream), *cache, hg::inverse_of(cache->page_size), kk, vv,
+  const bool many = int64_t(tokens) * cache->kv_heads >= hg::kMany;
+  const auto pick = [&](auto type, auto groups) {
+    using T = decltype(type);
+    constexpr int G = decltype(groups)::value;
+    return many ? hg::cache_write_kernel<T, G, 2> : hg::cache_write_kernel<T, G, 1>;
+  };
+  using Two = std::integral_constant<int, 2>;
+  using Four = std::integral_constant<int, 4>;
+  const auto kernel = bf16 ? (wide ? pick(__nv_bfloat16{}, Four{}) : pick(__nv_bfloat16{}, Two{})) : (wide ? pick(__half{}, Four{}) : pick(__half{}, Two{}));
+  hg::check(hg::launch_kernel(kernel, hg::token_blocks(*cache, tokens, many ? 2 : 1), dim3(hg::kThreads), 0, static_cast<cudaStream_t>(stream), *cache, hg::inverse_of(cache->page_size), kk, vv,
                               strides[0], strides[1], strides[2], strides[3], slots, tokens), "cache write");
   HG_CATCH
 }
@@ -159,9 +188,16 @@ int hg_cache_read(const hg_cache* cache, void* k, void* v, const int64_t* slots,
   if (!k || !v || !slots) throw std::runtime_error("Null argument to hg_cache_read");
   if (!hg::aligned16(k) || !hg::aligned16(v) || reinterpret_cast<uintptr_t>(slots) % 8) throw std::runtime_error("hg_cache_read: outputs must be aligned to 16 bytes");
   const bool bf16 = dtype == HG_DTYPE_BF16, wide = cache->head_dim == 128;
-  const auto kernel = bf16 ? (wide ? hg::cache_read_kernel<__nv_bfloat16, 4> : hg::cache_read_kernel<__nv_bfloat16, 2>)
-                           : (wide ? hg::cache_read_kernel<__half, 4> : hg::cache_read_kernel<__half, 2>);
-  hg::check(hg::launch_kernel(kernel, hg::token_blocks(*cache, tokens), dim3(hg::kThreads), 0, static_cast<cudaStream_t>(stream), *cache, hg::inverse_of(cache->page_size),
+  const bool many = int64_t(tokens) * cache->kv_heads >= hg::kMany;
+  const auto pick = [&](auto type, auto groups) {
+    using T = decltype(type);
+    constexpr int G = decltype(groups)::value;
+    return many ? hg::cache_read_kernel<T, G, 2> : hg::cache_read_kernel<T, G, 1>;
+  };
+  using Two = std::integral_constant<int, 2>;
+  using Four = std::integral_constant<int, 4>;
+  const auto kernel = bf16 ? (wide ? pick(__nv_bfloat16{}, Four{}) : pick(__nv_bfloat16{}, Two{})) : (wide ? pick(__half{}, Four{}) : pick(__half{}, Two{}));
+  hg::check(hg::launch_kernel(kernel, hg::token_blocks(*cache, tokens, many ? 2 : 1), dim3(hg::kThreads), 0, static_cast<cudaStream_t>(stream), *cache, hg::inverse_of(cache->page_size),
                               static_cast<uint16_t*>(k), static_cast<uint16_t*>(v), slots, tokens), "cache read");
   HG_CATCH
 }
