@@ -87,7 +87,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ float exp2_approx(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 __device__ __forceinline__ uint32_t half2_bits(float low, float high) {
   const __half2 h = __floats2half2_rn(low, high);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -184,13 +183,13 @@ __device__ __forceinline__ void meet(int count, float& m, float& l, float4& sum,
     const float before = m;
 #pragma unroll
     for (int j = 0; j < kMeet; ++j) m = fmaxf(m, y[j].x);
-    const float shrink = exp2_approx(before - m);
+    const float shrink = exp2_fast(before - m);
     l *= shrink;
     sum.x *= shrink; sum.y *= shrink; sum.z *= shrink; sum.w *= shrink;
 #pragma unroll
     for (int j = 0; j < kMeet; ++j) {
       if (first + j >= count) continue;
-      const float factor = exp2_approx(y[j].x - m);
+      const float factor = exp2_fast(y[j].x - m);
       l += y[j].y * factor;
       sum.x += x[j].x * factor; sum.y += x[j].y * factor; sum.z += x[j].z * factor; sum.w += x[j].w * factor;
     }
@@ -545,7 +544,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
 #pragma unroll
           for (int step = 4; step < 32; step <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, step));
           m = fmaxf(m, maximum[h]);
-          const float factor = exp2_approx(maximum[h] - m) * shrink;
+          const float factor = exp2_fast(maximum[h] - m) * shrink;
           maximum[h] = m;
           shift[h] = float(127 - value_scale) + kBias - m;
           weight[h] *= factor;
@@ -562,7 +561,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       }
       float2 probability[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) probability[i] = make_float2(exp2_approx(x[2 * i]), exp2_approx(x[2 * i + 1]));
+      for (int i = 0; i < 2; ++i) probability[i] = make_float2(exp2_fast(x[2 * i]), exp2_fast(x[2 * i + 1]));
       weight[0] += probability[0].x + probability[1].x;
       weight[1] += probability[0].y + probability[1].y;
 
@@ -631,7 +630,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       for (int j = 1; j < WARPS; ++j) m = fmaxf(m, maxima[j][h]);
 #pragma unroll
       for (int j = 0; j < WARPS; ++j) {
-        const float factor = exp2_approx(maxima[j][h] - m);
+        const float factor = exp2_fast(maxima[j][h] - m);
         const float4 part = *reinterpret_cast<const float4*>(&sums[j][h][d]);
         l += weights[j][h] * factor;
         sum.x += part.x * factor; sum.y += part.y * factor; sum.z += part.z * factor; sum.w += part.w * factor;

@@ -179,6 +179,10 @@ template <> struct Packed<__nv_bfloat16> {
   }
 };
 
+// 2^x and 1 / x to two units and one.
+__device__ __forceinline__ float exp2_fast(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float reciprocal_fast(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+
 // Two fp32 operations per instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;

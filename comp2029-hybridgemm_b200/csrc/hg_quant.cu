@@ -131,9 +131,6 @@ __device__ __forceinline__ void silu8(const uint4& g4, const uint4& u4, float (&
   product = make_uint4(dw[0], dw[1], dw[2], dw[3]);
 }
 
-__device__ __forceinline__ float exp2_fast(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-__device__ __forceinline__ float reciprocal_fast(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-
 // 2 N SwiGLU products by approximate exponentials and reciprocals, bit for bit silu8's.
 //
 // The gate's activation is rounded to 16 bits, so an fp32 value that is only nearly silu8's gives the same bits unless a
