@@ -21,6 +21,7 @@
 // of its whole group, and a rounding to 16 bits no longer hides the difference.  (37 sequences, codes against 64-bit arithmetic:
 // relative difference 0.015 with one product, none with two, 0.010 in fp32 arithmetic; 17.9 us and 18.8.)
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <mutex>
@@ -46,7 +47,7 @@ constexpr int kFew = 12288;          // tiles of all units that are left to clus
 constexpr int kHeld[2][5] = {{4000, 2000, 959, 479, 209}, {1000, 500, 222, 101, 47}};
 constexpr int kSmBytes = 228 << 10;  // shared memory of an SM
 constexpr float kBias = 7.f, kSlack = 4.f;   // P is kept in [0, 2^(kBias + 2 kSlack)]
-constexpr float kNone = -1e30f;      // maximum of nothing
+constexpr float kNone = -3e38f;      // maximum of nothing
 constexpr int kLeastScale = 24;      // values are summed under 2^-103 at least
 
 // How units come to blocks.  Few units (CLUSTER): a cluster of `split` blocks each, whose sums meet in shared memory.  Many (LINE):
@@ -55,15 +56,17 @@ constexpr int kLeastScale = 24;      // values are summed under 2^-103 at least
 // block than it begins in is added up by the one that it begins in, which comes to it last; the others come to their
 // parts of it first, write their sums to a slot and set a tag behind them, and the first one waits for the tags and takes them back.
 // It waits for blocks behind it alone, whose first parts wait for nothing, so the wait ends even where the device holds fewer blocks
-// than there are: all but one of them end.  A tag is 64 bits that a workspace holds by accident once in 2^64 slots, so it
-// needs no clearing, and no two calls share one.
-constexpr uint64_t kTag = 0x9d3f6ac1e57b2480ull;
+// than there are: all but one of them end.  A tag is 64 bits that a workspace holds by accident once in 2^64 slots, so that
+// it needs no clearing before a launch.  Every call has its own one, which a later call does not take for its tag where a wait was
+// given up, and replays of a captured one find the tags taken back.
+constexpr uint64_t kTag = 0x9d3f6ac1e57b2481ull;
 
 struct AttentionParams {
   hg_cache cache;
   hg_attention_call call;
   float* partial;       // LINE: [blocks][kHeadTile][head_dim + 2]: sums, maximum, sum of weights of a block's first part
   uint64_t* tags;       // LINE: [blocks]
+  uint64_t tag;
   int head_units;       // kv heads x chunks of kHeadTile heads
   int chunks, group;
   int split;            // CLUSTER: blocks of a unit, 1, 2, 4, 8 or 16
@@ -197,12 +200,12 @@ __device__ __forceinline__ void meet(int count, float& m, float& l, float4& sum,
 }
 
 // Waits until the tag is set; what was written before it is then visible.  False when it is not within about two seconds.
-__device__ __forceinline__ bool wait_for(const uint64_t* tag) {
+__device__ __forceinline__ bool wait_for(const uint64_t* at, uint64_t tag) {
   const long long start = clock64();
   for (uint32_t spin = 1;; ++spin) {
     uint64_t now;
-    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(now) : "l"(tag) : "memory");
-    if (now == kTag) return true;
+    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(now) : "l"(at) : "memory");
+    if (now == tag) return true;
     if ((spin & 63u) == 0) {
       __nanosleep(100);
       if (clock64() - start > kWaitLimitCycles) return false;
@@ -391,7 +394,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     // Queries as the second operand of the first product: column r is head r, rows the four elements at 32 g + 4 x.  A head's bf16 queries
     // become halves under a power of two that brings the largest to [2^14, 2^15).
     uint32_t q[GROUPS][2][2];
-    float to_log2[2];
+    float2 to_log2;
     {
       const uint16_t* const row = static_cast<const uint16_t*>(p.call.q) + seq * p.call.q_stride + int64_t(head0 + r) * kDim;
       uint32_t top = 0;
@@ -422,8 +425,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
               q[g][j][i] = half2_bits(pair.x * factor, pair.y * factor);
             }
       }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) to_log2[h] = __shfl_sync(0xffffffffu, back, 8 * c + 4 * h);
+      to_log2 = make_float2(__shfl_sync(0xffffffffu, back, 8 * c), __shfl_sync(0xffffffffu, back, 8 * c + 4));
     }
 
     float out[GROUPS][2][4];
@@ -434,7 +436,8 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
 #pragma unroll
         for (int i = 0; i < 4; ++i) out[g][h][i] = 0.f;
     // Heads 2c and 2c + 1.  Weights (of this lane's tokens) and values are summed over 2^(maximum + value_scale - 127 - kBias).
-    float maximum[2] = {kNone, kNone}, weight[2] = {0.f, 0.f}, shift[2] = {-kNone, -kNone};
+    float maximum[2] = {kNone, kNone}, weight[2] = {0.f, 0.f};
+    float2 shift = make_float2(-kNone, -kNone);
     int value_scale = kLeastScale;
 
     for (int t = begin + warp; t < end; t += WARPS) {
@@ -493,6 +496,9 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
           sum[i] = g == 0 ? mul2(by2, part2) : fma2(by2, part2, sum[i]);
         }
       }
+      // The logarithms of the weights are rounded before the maximum is taken off, so the largest is off by nothing, whatever its size.
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sum[i] = mul2(sum[i], to_log2);
       const float s[4] = {sum[0].x, sum[0].y, sum[1].x, sum[1].y};
       uint32_t v[4][GROUPS];                                 // tokens value_token, odd_token and those eight behind: elements 32 g + 4 r ...
 #pragma unroll
@@ -519,9 +525,9 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
           }
         }
       }
-      float x[4], scale[2][GROUPS], top = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = s[i] * to_log2[i & 1] + shift[i & 1];
+      float scale[2][GROUPS], top = 0.f;
+      const float2 first = add2(sum[0], shift), second = add2(sum[1], shift);
+      float x[4] = {first.x, first.y, second.x, second.y};
       if (!whole_tile) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -540,17 +546,17 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
         value_scale = new_scale;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float m = fmaxf(seen[0] ? s[h] * to_log2[h] : kNone, seen[1] ? s[h + 2] * to_log2[h] : kNone);
+          float m = fmaxf(seen[0] ? s[h] : kNone, seen[1] ? s[h + 2] : kNone);
 #pragma unroll
           for (int step = 4; step < 32; step <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, step));
           m = fmaxf(m, maximum[h]);
           const float factor = exp2_fast(maximum[h] - m) * shrink;
           maximum[h] = m;
-          shift[h] = float(127 - value_scale) + kBias - m;
+          (h ? shift.y : shift.x) = float(127 - value_scale) + kBias - m;
           weight[h] *= factor;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            x[h + 2 * i] = seen[i] ? s[h + 2 * i] * to_log2[h] + shift[h] : -INFINITY;
+            x[h + 2 * i] = seen[i] ? s[h + 2 * i] + (h ? shift.y : shift.x) : -INFINITY;
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
               out[g][i][h] *= factor;
@@ -619,7 +625,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     const int others = LINE && begins && !ends ? int((position + cost - 1) / share) - int(blockIdx.x) : 0;
     if (others) {
       for (int i = threadIdx.x; i < others; i += kThreads)
-        if (!wait_for(p.tags + blockIdx.x + 1 + i)) given_up = 1;
+        if (!wait_for(p.tags + blockIdx.x + 1 + i, p.tag)) given_up = 1;
       __syncthreads();
     }
     for (int i = threadIdx.x; i < heads * kDim / 4; i += kThreads) {   // whole groups of eight lanes
@@ -660,7 +666,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     if constexpr (LINE) {
       if (!begins) {
         __syncthreads();
-        if (threadIdx.x == 0) asm volatile("fence.acq_rel.gpu;\n st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p.tags + blockIdx.x), "l"(kTag) : "memory");
+        if (threadIdx.x == 0) asm volatile("fence.acq_rel.gpu;\n st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p.tags + blockIdx.x), "l"(p.tag) : "memory");
       } else if (others) {
         for (int i = threadIdx.x; i < others; i += kThreads) p.tags[blockIdx.x + 1 + i] = 0;
       }
@@ -835,10 +841,12 @@ int hg_attention(const hg_cache* cache, const hg_attention_call* call, int dtype
     throw std::runtime_error("hg_attention: pointers must be aligned to 16 bytes and q_stride to 8 elements");
   const hg::Split s = hg::split_of(*cache, a.seqs, a.heads, a.table_width, a.window);
   const uint32_t page_tiles = uint32_t(cache->page_size / hg::kTile);
-  hg::AttentionParams p{*cache, a, nullptr, nullptr, s.head_units, s.chunks, a.heads / cache->kv_heads, s.split, s.ring, page_tiles,
+  hg::AttentionParams p{*cache, a, nullptr, nullptr, 0, s.head_units, s.chunks, a.heads / cache->kv_heads, s.split, s.ring, page_tiles,
                         uint32_t(((uint64_t(1) << 32) + page_tiles - 1) / page_tiles)};
   if (s.line) {
     if (!a.workspace) throw std::runtime_error("hg_attention: a workspace is needed");
+    static std::atomic<uint64_t> calls{0};
+    p.tag = hg::kTag * (2 * calls.fetch_add(1, std::memory_order_relaxed) + 1);   // odd numbers: none is zero, and no two are alike for 2^63 calls
     p.tags = static_cast<uint64_t*>(a.workspace);
     p.partial = reinterpret_cast<float*>(p.tags + (s.blocks + 1 & ~1));
   }

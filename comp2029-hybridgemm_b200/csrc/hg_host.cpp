@@ -13,6 +13,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -175,6 +176,8 @@ struct Unlocked {
 // Operands of `DualLinear.linear`: null, or what an epilogue takes.
 struct Added { const at::Tensor *bias, *residual; int activation; };
 
+// A gradient would be asked of it: the calls have none, and Python says so.
+bool differentiated(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
 bool sixteen_bits(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
 bool aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
 int dtype_of(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? HG_DTYPE_BF16 : HG_DTYPE_F16; }
@@ -201,15 +204,15 @@ PyObject* forward_checked(PyObject* self, const at::Tensor& x, long math, const 
   hg_epilogue epilogue{};
   if (added) {
     const auto type = r->output.dtype().toScalarType();
-    if (r->explicit_schedule || x.requires_grad()) Py_RETURN_NONE;
+    if (r->explicit_schedule || differentiated(x)) Py_RETURN_NONE;
     if (const at::Tensor* bias = added->bias) {
-      if (bias->device() != r->device || bias->scalar_type() != type || bias->dim() != 1 || bias->size(0) != r->outputs || !bias->is_contiguous() || bias->requires_grad())
+      if (bias->device() != r->device || bias->scalar_type() != type || bias->dim() != 1 || bias->size(0) != r->outputs || !bias->is_contiguous() || differentiated(*bias))
         Py_RETURN_NONE;
       epilogue.bias = bias->const_data_ptr();
     }
     if (const at::Tensor* residual = added->residual) {
       if (residual->device() != r->device || residual->scalar_type() != type || residual->dim() != 2 || residual->size(0) != r->tokens ||
-          residual->size(1) != r->outputs || residual->stride(1) != 1 || residual->requires_grad())
+          residual->size(1) != r->outputs || residual->stride(1) != 1 || differentiated(*residual))
         Py_RETURN_NONE;
       epilogue.residual = residual->const_data_ptr();
       epilogue.residual_stride = residual->stride(0);
@@ -322,10 +325,10 @@ PyObject* tuple_of(std::initializer_list<PyObject*> items) {
 // A 16-bit matrix like x: contiguous rows aligned to 16 bytes.
 bool rows_like(const at::Tensor& t, const at::Tensor& x) {
   return t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.dim() == 2 && t.size(0) == x.size(0) && t.size(1) == x.size(1) &&
-         t.stride(1) == 1 && (t.size(0) <= 1 || t.stride(0) % 8 == 0) && aligned(t) && !t.requires_grad();
+         t.stride(1) == 1 && (t.size(0) <= 1 || t.stride(0) % 8 == 0) && aligned(t) && !differentiated(t);
 }
 bool vector_like(const at::Tensor& t, const at::Tensor& x) {
-  return t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.dim() == 1 && t.size(0) == x.size(1) && t.is_contiguous() && aligned(t) && !t.requires_grad();
+  return t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.dim() == 1 && t.size(0) == x.size(1) && t.is_contiguous() && aligned(t) && !differentiated(t);
 }
 
 // norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, packed)
@@ -416,7 +419,7 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
       const at::Tensor& t = i ? v : k;
       if (t.device() != data.device() || !sixteen_bits(t) || t.scalar_type() != k.scalar_type() || t.dim() != 3 || t.size(0) != slots.size(0) ||
           t.size(1) != cache.kv_heads || t.size(2) != head_dim || t.stride(2) != 1 || t.stride(0) % 4 || t.stride(1) % 4 ||
-          reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 8 || t.requires_grad())
+          reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 8 || differentiated(t))
         Py_RETURN_NONE;
       strides[2 * i] = t.stride(0);
       strides[2 * i + 1] = t.stride(1);
@@ -475,7 +478,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     hg_cache cache;
     if (!cache_of(data, page_size, head_dim, &cache) || q.device() != data.device() || !sixteen_bits(q) || q.dim() != 3 || q.size(2) != head_dim || !q.size(0) ||
         !q.size(1) || q.size(1) % cache.kv_heads || q.stride(2) != 1 || (q.size(1) > 1 && q.stride(1) != head_dim) || (q.size(0) > 1 && q.stride(0) % 8) ||
-        !aligned(q) || q.requires_grad() || (packed && q.size(1) * head_dim % 128) || q.size(0) > 0x7fffffff || q.size(1) > 0x7fffff)
+        !aligned(q) || differentiated(q) || (packed && q.size(1) * head_dim % 128) || q.size(0) > 0x7fffffff || q.size(1) > 0x7fffff)
       Py_RETURN_NONE;
     const int64_t seqs = q.size(0), heads = q.size(1);
     if (table.device() != data.device() || table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != seqs || (table.size(1) > 1 && table.stride(1) != 1) ||

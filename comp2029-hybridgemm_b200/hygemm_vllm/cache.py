@@ -20,7 +20,7 @@ import ctypes as C
 import torch
 
 from . import native
-from .native import DTYPES, _on_device, _stream, check, library, scale_size
+from .native import DTYPES, _differentiated, _on_device, _stream, check, library, scale_size
 
 
 class Cache(C.Structure):
@@ -86,7 +86,7 @@ class PagedCache:
             if x.numel() and (x.stride(2) != 1 or x.data_ptr() % 8 or x.stride(0) % 4 or x.stride(1) % 4):
                 raise ValueError("PagedCache.write requires contiguous heads aligned to 8 bytes")
         self._slots(slots)
-        if k.requires_grad or v.requires_grad:
+        if _differentiated(k, v):
             raise ValueError("PagedCache.write has no gradient")
         if not shape[0]:
             return
@@ -146,7 +146,7 @@ class PagedCache:
         seqs, heads, _ = q.shape
         if seqs and (q.stride(2) != 1 or (heads > 1 and q.stride(1) != self.head_dim) or (seqs > 1 and q.stride(0) % 8) or q.data_ptr() % 16):
             raise ValueError("PagedCache.attention requires contiguous query rows aligned to 16 bytes")
-        if q.requires_grad:
+        if _differentiated(q):
             raise ValueError("PagedCache.attention has no gradient")
         if not (page_table.device == device and page_table.dtype == torch.int32 and page_table.ndim == 2 and page_table.shape[0] == seqs
                 and (page_table.stride(1) == 1 or page_table.shape[1] <= 1)):
@@ -175,7 +175,7 @@ class PagedCache:
             workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
             call = AttentionCall(q.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), out.data_ptr() if out is not None else None,
                                  codes.data_ptr() if packed else None, sf.data_ptr() if packed else None,
-                                 sums.data_ptr() if lse else None, workspace.data_ptr() if size else None, q.stride(0),
+                                 sums.data_ptr() if lse else None, workspace.data_ptr() if size else None, q.stride(0) if rows > 1 else 0,
                                  page_table.stride(0), rows, heads, width, window,
                                  self.head_dim ** -0.5 if scale is None else scale)
             with _on_device(device):

@@ -176,6 +176,11 @@ def _on_device(device):
     return _HERE if torch._C._cuda_getDevice() == device.index else _switched(device)
 
 
+def _differentiated(*tensors) -> bool:
+    """Whether a gradient would be asked of one of them: the calls of this package are forward only."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def pack(x: torch.Tensor, fp4: bool = False):
     """Quantise `[rows,K]` fp16/bf16 to MX codes + padded E8M0 scales (reference: native.py:40-50).
 
@@ -301,7 +306,7 @@ class DualLinear:
             raise ValueError("HyGEMM input shape/device does not match its weights")
         tokens = x.shape[0]
         epilogue = self._epilogue(tokens, bias, activation, residual, x)
-        if tokens and _host is not None and not PACK_MODE and tokens not in self._ready and not x.requires_grad:
+        if tokens and _host is not None and not PACK_MODE and tokens not in self._ready:
             with _on_device(x.device):
                 self._prepare(x)   # the calls that follow go through the host extension
         y = torch.empty((tokens, self.outputs), dtype=self.dtype, device=x.device)
@@ -323,17 +328,21 @@ class DualLinear:
         """The checked operands of an epilogue, as the library takes them."""
         if activation not in ACTIVATIONS:
             raise ValueError(f"HyGEMM epilogue activation must be one of {sorted(a for a in ACTIVATIONS if a)}")
-        if self.plans or self.low_id or self.high_id or not self._tensor_core():
+        if not self.takes_epilogue():
             raise ValueError("HyGEMM epilogue requires a layer with the automatic schedule")
         if bias is not None and not (bias.device == x.device and bias.dtype == self.dtype and bias.shape == (self.outputs,) and bias.is_contiguous()):
             raise ValueError("HyGEMM epilogue requires a contiguous bias [outputs] of the layer's type and device")
         if residual is not None and not (residual.device == x.device and residual.dtype == self.dtype
                                          and residual.shape == (tokens, self.outputs) and (residual.stride(1) == 1 or self.outputs == 1)):
             raise ValueError("HyGEMM epilogue requires a residual [tokens, outputs] of the layer's type and device with contiguous rows")
-        if any(t is not None and t.requires_grad for t in (x, bias, residual)):
+        if _differentiated(x, bias, residual):
             raise ValueError("HyGEMM layers have no gradient")
         return Epilogue(None if bias is None else bias.data_ptr(), None if residual is None or not tokens else residual.data_ptr(),
                         0 if residual is None else residual.stride(0), ACTIVATIONS[activation])
+
+    def takes_epilogue(self) -> bool:
+        """Whether `linear` and `run_packed` take bias, activation and residual: the automatic schedule, on the tensor-core launch."""
+        return not (self.plans or self.low_id or self.high_id) and self._tensor_core()
 
     def silu_linear(self, x, math):
         """This layer on SwiGLU of `x` = gate||up `[tokens, 2K]`: `producer.silu_pack` followed by `run_packed`."""

@@ -3,7 +3,8 @@
 `hygemm_vllm::linear` and `hygemm_vllm::linear_silu` keep the reference's
 schemas (quantization.py:18-25, producer.py:27-40 of the reference): the layer
 runtime is looked up by an integer handle in `_runtimes`, nothing is mutated,
-and the fake implementations give shape/dtype for tracing.
+and the fake implementations give shape/dtype for tracing.  `hygemm_vllm::linear_epilogue` adds bias, activation and
+residual (`DualLinear.linear`).
 
 An eager call of a custom op costs about as much host time as the layer itself, so calling `linear` or `linear_silu` on an
 ordinary tensor with nothing watching goes straight to the layer.  Everything else goes through the dispatcher: tracing,
@@ -11,6 +12,8 @@ modes, functorch transforms, profiling, tensor subclasses and wrappers, tensors 
 and say so in the backward pass).
 """
 from __future__ import annotations
+
+from typing import Optional
 
 import torch
 
@@ -80,5 +83,25 @@ def _define(name, function, fake):
     return op
 
 
+def _linear_epilogue(x: torch.Tensor, handle: int, outputs: int, bias: Optional[torch.Tensor], activation: str,
+                     residual: Optional[torch.Tensor]) -> torch.Tensor:
+    return _runtimes[handle].linear(x, bias, activation, residual)
+
+
+def _linear_epilogue_fake(x, handle, outputs, bias, activation, residual):
+    return x.new_empty((x.shape[0], outputs))
+
+
+class _EpilogueOp(_Op):
+    """The short way is for calls all of whose tensors are ordinary."""
+
+    def __call__(self, x, handle, outputs, bias, activation, residual):
+        if _plain(x) and all(t is None or _plain(t) for t in (bias, residual)):
+            return self.direct(x, handle, outputs, bias, activation, residual)
+        return torch.library.CustomOpDef.__call__(self, x, handle, outputs, bias, activation, residual)
+
+
 linear = _define("linear", _linear, _linear_fake)
 linear_silu = _define("linear_silu", _linear_silu, _linear_silu_fake)
+linear_epilogue = _define("linear_epilogue", _linear_epilogue, _linear_epilogue_fake)
+linear_epilogue.__class__ = _EpilogueOp

@@ -16,13 +16,18 @@ random-init models whose weights only exist after loading.
 """
 from __future__ import annotations
 
+import os
+
 import torch
 from vllm.model_executor.layers.linear import LinearBase, LinearMethodBase, UnquantizedLinearMethod
 from vllm.model_executor.layers.quantization import register_quantization_config
 from vllm.model_executor.layers.quantization.base_config import QuantizationConfig
 
 from . import tp
-from .ops import _runtimes, linear, register_runtime  # noqa: F401  (`_runtimes` is read by producer/worker code)
+from .ops import _runtimes, linear, linear_epilogue, register_runtime  # noqa: F401  (`_runtimes` is read by producer/worker code)
+
+# HYGEMM_FUSE_BIAS=1: a layer's bias is added in the GEMM's fp32 epilogue (one rounding instead of two, no second kernel).
+FUSE_BIAS = os.environ.get("HYGEMM_FUSE_BIAS", "0") == "1"
 
 _FUSED = {".qkv_proj": ("q", "k", "v"), ".gate_up_proj": ("gate", "up")}
 
@@ -169,9 +174,13 @@ class MixedLinearMethod(LinearMethodBase):
     # -- forward --------------------------------------------------------------------------------
     def apply(self, layer, x, bias=None):
         lead = x.shape[:-1]
-        y = linear(x.reshape(-1, self.k).contiguous(), self.handle, self.outputs)
-        if bias is not None:
-            y = y + bias
+        x = x.reshape(-1, self.k).contiguous()
+        if bias is not None and FUSE_BIAS and self.runtime.takes_epilogue():
+            y = linear_epilogue(x, self.handle, self.outputs, bias.detach(), "none", None)
+        else:
+            y = linear(x, self.handle, self.outputs)
+            if bias is not None:
+                y = y + bias
         return y.reshape(*lead, self.outputs)
 
     def reduce(self, y):
