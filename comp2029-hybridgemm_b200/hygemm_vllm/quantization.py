@@ -175,7 +175,7 @@ class MixedLinearMethod(LinearMethodBase):
     def apply(self, layer, x, bias=None):
         lead = x.shape[:-1]
         x = x.reshape(-1, self.k).contiguous()
-        if bias is not None and FUSE_BIAS and self.runtime.takes_epilogue():
+        if bias is not None and FUSE_BIAS and bias.dtype == x.dtype and bias.is_contiguous() and self.runtime.takes_epilogue():
             y = linear_epilogue(x, self.handle, self.outputs, bias.detach(), "none", None)
         else:
             y = linear(x, self.handle, self.outputs)
