@@ -39,9 +39,14 @@ constexpr int kWarps = 4, kWideWarps = 12;   // of a block; of one that has an S
 constexpr int kMostRing = 4;        // tiles of a warp in shared memory or on their way there, at most
 constexpr int kBlocksPerSm = 4, kLineBlocksPerSm = 3;   // of kWarps; of a line of no more units than that
 constexpr int kWhole = 16;           // sequences of no more tiles are not split
-constexpr int kUnitCost = 16;        // cost of a unit beside its tiles, in tiles
-constexpr int kLeastShare = 24;      // a block's share of the cost, where there is less for all blocks
-constexpr int kFew = 12288;          // tiles of all units that are left to clusters, whatever part of the device these fill
+// Costs in tiles.  A unit costs kUnitCost beside its tiles, units that are split kSplitCost (in a block of kWarps), and a block takes at
+// least kLeastShare.
+constexpr int kUnitCost = 16, kSplitCost = 36, kLeastShare = 24;
+// Tiles of all units up to which they are left to clusters: kFew where the clusters fill less than three quarters of the device, kMuch
+// otherwise.  A cluster's blocks take equal parts of one unit, so the longest unit sets the time; a line has a slower beginning and end.
+// Cluster and line, us, 4 kv heads of 128: 1 x 32000 tokens 16.8, 18.3; 4 x 32768 52, 32; 8 x 4000 12.8, 16.5, 8 of 10 to 4000 10.5, 12.5;
+// 8 x 16000 28.4, 32.1, 8 of 10 to 16000 26.4, 17.1; 36 x 4000 28.8, 30.4, 36 of 10 to 4000 25.0, 20.7.
+constexpr int kFew = 12288, kMuch = 24576;
 // Clusters of 1, 2, 4, 8 and 16 blocks that a device holds at once, per thousand SMs: blocks of kWarps (whose SMs hold several), and of
 // kWideWarps.  GPCs differ in their SMs, so it is not a matter of division (148 SMs: 592, 296, 142, 71 and 31; 148, 74, 33, 15 and 7).
 constexpr int kHeld[2][5] = {{4000, 2000, 959, 479, 209}, {1000, 500, 222, 101, 47}};
@@ -67,6 +72,9 @@ struct AttentionParams {
   float* partial;       // LINE: [blocks][kHeadTile][head_dim + 2]: sums, maximum, sum of weights of a block's first part
   uint64_t* tags;       // LINE: [blocks]
   uint64_t tag;
+  int least, more;      // LINE: units of a block, and blocks that have one more
+  float by_blocks;      // LINE: 1 / blocks, rounded up
+  int table_lines;      // 128-byte lines of a row of the table
   int head_units;       // kv heads x chunks of kHeadTile heads
   int chunks, group;
   int split;            // CLUSTER: blocks of a unit, 1, 2, 4, 8 or 16
@@ -94,8 +102,17 @@ __device__ __forceinline__ uint32_t half2_bits(float low, float high) {
   const __half2 h = __floats2half2_rn(low, high);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// 2^(byte - 127) of byte g; 0 for byte 0.
-__device__ __forceinline__ float scale_of(uint32_t word, int g) { return __uint_as_float(__byte_perm(word, 0, 0x0444 | (g << 12)) >> 1); }
+// 2^(byte - 127) of a pair of bytes, as bf16, and of one of them.
+__device__ __forceinline__ uint32_t two_scales(uint32_t bytes) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(r) : "h"(uint16_t(bytes)));
+  return r;
+}
+__device__ __forceinline__ float scale_of(uint32_t pair, int g) { return __uint_as_float(g & 1 ? pair & 0xffff0000u : pair << 16); }
+__device__ __forceinline__ uint32_t max_pairs(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
 __device__ __forceinline__ float power_of(int biased) { return __uint_as_float(uint32_t(biased) << 23); }
 
 __device__ __forceinline__ uint4 shared_16(uint32_t at) {
@@ -253,6 +270,13 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
+  // Lengths and tables come as far as L2 while the kernel in front ends (a call from cold memory then has its first tile 0.7 us earlier);
+  // what they hold is read behind the wait.
+  {
+    const int at = int(blockIdx.x * kThreads + threadIdx.x), row = at / p.table_lines;
+    if (threadIdx.x * 32 < p.call.seqs) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.call.lengths + threadIdx.x * 32));
+    if (row < p.call.seqs) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.call.table + row * p.call.table_stride + (at - row * p.table_lines) * 32));
+  }
   // Loads below are ordinary ones: the kernel in front may still be writing the cache when this one starts, so the data is not
   // read-only for its duration.
   pdl_wait();
@@ -273,6 +297,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   if constexpr (LINE) {
     __shared__ int64_t sums_of[WARPS];
     __shared__ int found[2], largest_of[WARPS];
+    const unsigned blocks = gridDim.x;
     auto tiles_of = [&](int i) {
       if (i >= p.call.seqs) return -kUnitCost;
       const Span s = span_of(p, i);
@@ -292,14 +317,15 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) largest = max(largest, largest_of[i]);
     largest += kUnitCost;
-    share = max(int64_t(kLeastShare), (s.all + gridDim.x - 1) / gridDim.x);
-    const int64_t units = int64_t(p.call.seqs) * p.head_units;
-    // No unit is split where none is much longer than the others and their number fits that of the blocks.
-    const int64_t rounds = (units + gridDim.x - 1) / gridDim.x;
-    whole = units * largest * 4 <= s.all * 5 && (units >= gridDim.x ? units * 5 >= rounds * gridDim.x * 4 : units * 3 >= gridDim.x);
+    share = max(int64_t(kLeastShare), int64_t(float(s.all) * p.by_blocks) + 1);   // at least s.all / blocks
+    // No unit is split where the longest of them, as many as a block gets, cost no more than an equal share and a split.  Whole and split, us:
+    // 64 x 500 tokens of 4 heads 14.8, 18.9, 64 x 2000 39.9, 35.1; 40 x 4000 72, 38; 96 x 4000 75.1, 77.5; 128 x 2000 53.2, 57.2.
+    whole = int64_t(largest) * (p.least + (p.more > 0)) <= share + kSplitCost * WARPS / kWarps;
     if (whole) {
-      position = (blockIdx.x * units + gridDim.x - 1) / gridDim.x;   // units position ..., so that blocks with one more are spread over the SMs
-      remaining = ((blockIdx.x + 1) * units + gridDim.x - 1) / gridDim.x - position;
+      // blocks with one unit more are spread over the SMs
+      const unsigned ahead = (blockIdx.x * unsigned(p.more) + blocks - 1) / blocks;
+      position = int64_t(blockIdx.x) * p.least + ahead;
+      remaining = p.least + int((blockIdx.x * unsigned(p.more) + p.more + blocks - 1) / blocks - ahead);
       if (remaining <= 0) return;
     } else {
       position = blockIdx.x * share;
@@ -478,6 +504,14 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       }
       // Scores: tokens my_token and my_token + 8, heads 2c and 2c + 1.
       float2 sum[2];
+      uint32_t key_scales[2][GROUPS / 2], value_scales[2][GROUPS / 2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < GROUPS / 2; ++j) {
+          key_scales[i][j] = two_scales(ks[i] >> (16 * j));
+          value_scales[i][j] = two_scales(vs[i] >> (16 * j));
+        }
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
         float part[4];
@@ -491,7 +525,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float by = scale_of(ks[i], g);
+          const float by = scale_of(key_scales[i][g / 2], g);
           const float2 by2 = make_float2(by, by), part2 = make_float2(part[2 * i], part[2 * i + 1]);
           sum[i] = g == 0 ? mul2(by2, part2) : fma2(by2, part2, sum[i]);
         }
@@ -525,7 +559,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
           }
         }
       }
-      float scale[2][GROUPS], top = 0.f;
+      float scale[2][GROUPS];
       const float2 first = add2(sum[0], shift), second = add2(sum[1], shift);
       float x[4] = {first.x, first.y, second.x, second.y};
       if (!whole_tile) {
@@ -536,7 +570,10 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) top = fmaxf(top, scale[i][g] = scale_of(vs[i], g));
+        for (int i = 0; i < 2; ++i) scale[i][g] = scale_of(value_scales[i][g / 2], g);
+      uint32_t tops = max_pairs(value_scales[0][0], value_scales[1][0]);
+      if constexpr (GROUPS == 4) tops = max_pairs(tops, max_pairs(value_scales[0][1], value_scales[1][1]));
+      const float top = fmaxf(scale_of(tops, 0), scale_of(tops, 1));
 
       // A new maximum, or larger scales of the values, is taken up only when a weight could leave the range of a half.
       const bool rescale = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > float(127 - value_scale) + (kBias + kSlack) || top > power_of(value_scale) * 16.f;
@@ -622,7 +659,11 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     __syncthreads();
     const bool begins = from == 0, ends = to == cost;   // whole units: both
     // Where the unit ends in a block behind this one, this block waits for the parts of the blocks up to there.
-    const int others = LINE && begins && !ends ? int((position + cost - 1) / share) - int(blockIdx.x) : 0;
+    int others = 0;
+    if (LINE && begins && !ends) {
+      const int64_t last = position + cost - 1 - blockIdx.x * share;   // of the unit, behind this block's first place
+      others = share >> 31 ? int(last >= share) : int(uint32_t(last) / uint32_t(share));
+    }
     if (others) {
       for (int i = threadIdx.x; i < others; i += kThreads)
         if (!wait_for(p.tags + blockIdx.x + 1 + i, p.tag)) given_up = 1;
@@ -739,11 +780,16 @@ Split split_of(const hg_cache& c, int seqs, int heads, int table_width, int wind
       s.per_sm = wide ? 1 : kBlocksPerSm;
       s.split = split;
     }
-  s.line = longest > kWhole && (s.units > sms || (s.units * longest > kFew && most * 4 < int64_t(sms) * kWideWarps * 3));
+  // More units than SMs, or much work: a line.
+  s.line = longest > kWhole && (s.units > sms || s.units * longest > kMuch || (s.units * longest > kFew && most * 4 < int64_t(sms) * kWideWarps * 3));
   s.blocks = int(s.units * s.split);
   if (s.line) {
-    s.warps = kWarps;
-    s.per_sm = s.units <= sms * kLineBlocksPerSm ? kLineBlocksPerSm : kBlocksPerSm;
+    // Few units have many parts each: a wide block to an SM makes these a third as many, and its warps end together (4 x 32768: 31.9 us; three
+    // blocks 34.5).  With more units, blocks that begin and end one at different times cover for one another (37 of 1 to 4099: 18.3;
+    // one wide block 26.1).
+    const bool wide = s.units <= sms;
+    s.warps = wide ? kWideWarps : kWarps;
+    s.per_sm = wide ? 1 : s.units <= sms * kLineBlocksPerSm ? kLineBlocksPerSm : kBlocksPerSm;
     s.split = 1;
     s.blocks = int(std::min<int64_t>(sms * s.per_sm, (s.units * (longest + kUnitCost) + kLeastShare - 1) / kLeastShare));
   }
@@ -841,12 +887,15 @@ int hg_attention(const hg_cache* cache, const hg_attention_call* call, int dtype
     throw std::runtime_error("hg_attention: pointers must be aligned to 16 bytes and q_stride to 8 elements");
   const hg::Split s = hg::split_of(*cache, a.seqs, a.heads, a.table_width, a.window);
   const uint32_t page_tiles = uint32_t(cache->page_size / hg::kTile);
-  hg::AttentionParams p{*cache, a, nullptr, nullptr, 0, s.head_units, s.chunks, a.heads / cache->kv_heads, s.split, s.ring, page_tiles,
+  hg::AttentionParams p{*cache, a, nullptr, nullptr, 0, 0, 0, 0.f, std::max(1, a.table_width / 32 + (a.table_width % 32 ? 1 : 0)), s.head_units, s.chunks, a.heads / cache->kv_heads, s.split, s.ring, page_tiles,
                         uint32_t(((uint64_t(1) << 32) + page_tiles - 1) / page_tiles)};
   if (s.line) {
     if (!a.workspace) throw std::runtime_error("hg_attention: a workspace is needed");
     static std::atomic<uint64_t> calls{0};
     p.tag = hg::kTag * (2 * calls.fetch_add(1, std::memory_order_relaxed) + 1);   // odd numbers: none is zero, and no two are alike for 2^63 calls
+    p.least = int(s.units / s.blocks);
+    p.more = int(s.units % s.blocks);
+    p.by_blocks = 1.000001f / float(s.blocks);
     p.tags = static_cast<uint64_t*>(a.workspace);
     p.partial = reinterpret_cast<float*>(p.tags + (s.blocks + 1 & ~1));
   }
@@ -855,6 +904,7 @@ int hg_attention(const hg_cache* cache, const hg_attention_call* call, int dtype
     using T = decltype(type);
     constexpr int G = decltype(groups)::value;
     constexpr bool E = decltype(exact)::value;
+    if (s.line && s.warps == hg::kWideWarps) return hg::launch_attention<T, G, hg::kWideWarps, 1, true, E>;
     if (s.line)
       return s.per_sm == hg::kLineBlocksPerSm ? hg::launch_attention<T, G, hg::kWarps, hg::kLineBlocksPerSm, true, E> : hg::launch_attention<T, G, hg::kWarps, hg::kBlocksPerSm, true, E>;
     return s.warps == hg::kWideWarps ? hg::launch_attention<T, G, hg::kWideWarps, 1, false, E> : hg::launch_attention<T, G, hg::kWarps, hg::kBlocksPerSm, false, E>;

@@ -29,6 +29,10 @@ PLANS = [
     (14, 7, 128, 16, ragged(14, 260, 1000), 0),
     (16, 8, 64, 16, ragged(18, 260, 2000), 0),
     (8, 8, 64, 16, [32000], 0),                            # one sequence that fills the device
+    (8, 4, 64, 16, ragged(16, 100, 9000), 0),              # few long ones, over a line of wide blocks
+    (20, 2, 128, 32, ragged(30, 0, 5000), 0),
+    (4, 2, 128, 16, [6000] * 70, 0),                       # as many as such blocks, alike
+    (8, 4, 64, 16, ragged(20, 1, 20000), 6000),
     (28, 4, 128, 16, ragged(64, 10, 1000), 0),             # a line of blocks, three to an SM
     (8, 4, 64, 48, ragged(90, 0, 800), 0),
     (2, 1, 64, 16, [200000] + [3] * 159, 0),               # one sequence over hundreds of blocks
