@@ -42,7 +42,7 @@ def build_host_extension(force: bool = False) -> Path:
     extension.parent.mkdir(exist_ok=True)
     cmd = ["g++", "-O2", "-std=c++20", "-fPIC", "-shared", "-Wall", "-I", sysconfig.get_paths()["include"],
            *[a for p in include_paths("cuda") for a in ("-isystem", p)], str(HOST_SOURCE), "-o", str(extension),
-           *["-L" + p for p in library_paths("cuda")], "-lc10", "-lc10_cuda", "-lcudart", "-ltorch_cpu", "-ltorch_python"]
+           *["-L" + p for p in library_paths("cuda")], "-lc10", "-lc10_cuda", "-lcudart", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode:
         sys.stderr.write(result.stdout + result.stderr)

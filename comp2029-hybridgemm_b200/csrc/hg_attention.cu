@@ -3,9 +3,9 @@
 //   s_t = scale q . k_t      p_t = exp(s_t - max s)      out = sum_t p_t v_t / sum_t p_t
 //
 // One pass over the cache with a running maximum and sum, in one launch.  A unit of work is a sequence, a kv head and up to eight of its
-// query heads.  A cluster of blocks takes one unit, each block a run of its 16-token tiles, each warp of a block every fourth of these;
-// the blocks' sums meet in shared memory.  A tile comes in by TMA, a few tiles ahead, into a ring that the warp has for itself, and
-// goes from there into the fragments of two matrix products,
+// query heads.  A block takes a run of a unit's 16-token tiles, and each of its warps every fourth (or twelfth) of these; sums of warps
+// meet in shared memory, of blocks there or in a workspace.  A tile comes in by TMA, a few tiles ahead, into a ring that the warp has for
+// itself, and goes from there into the fragments of two matrix products,
 //   S^T [16 tokens, 8 heads]     = K [16 tokens, d]   Q^T [d, 8 heads]       (m16n8k16, one accumulator for every scale group of 32 d)
 //   O^T [16 d, 8 heads]          = V^T [16 d, tokens] P^T [tokens, 8 heads]
 // so that the heads fill the narrow side of an instruction, whatever their number, and the cache its wide one.  (tcgen05 would
@@ -14,12 +14,17 @@
 // those of the keys multiply a group's partial sum, those of the values the probabilities, once for every group, before these are
 // rounded to halves.
 //
+// What bounds it: bytes of the cache, and nearly as soon a warp's way through a tile (about 435 instructions for 4224 bytes, issued in half
+// of the slots, with the ALU pipe busy as long; from L2 an SM keeps up with some 24 bytes a clock, and memory delivers 23.6).  28 heads on 4 of 128, bf16: 128 sequences of 1024 to 1150 tokens
+// 31.7 us (0.72 of the measured copy rate), 128 x 4000 about 94 us (0.88), 4 x 32768 32.0 us (0.66); 1 x 1000 5.2 us, of which launch, three
+// dependent loads and two meetings of blocks are all but 0.2.
+//
 // Roundings: q keeps its 16 bits (a head's bf16 queries become halves under a power of two, which keeps eight bits of all that is
 // not 2^-29 of the largest).  P times the scale of its values is rounded to 11 bits (2^-11 of each weight at most), held
 // between 2^-32 and 2^8 of the largest so far by a bias of 2^7 and lazy rescaling.  Sums, maxima and outputs are fp32.  Where the output
 // is quantised (EXACT) what the rounding of P left goes through a second product: an output beside the border of two scales changes the codes
 // of its whole group, and a rounding to 16 bits no longer hides the difference.  (37 sequences, codes against 64-bit arithmetic:
-// relative difference 0.015 with one product, none with two, 0.010 in fp32 arithmetic; 17.9 us and 18.8.)
+// relative difference 0.015 with one product, none with two, 0.010 in fp32 arithmetic; 17.9 us and 18.3.)
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -44,8 +49,8 @@ constexpr int kWhole = 16;           // sequences of no more tiles are not split
 constexpr int kUnitCost = 16, kSplitCost = 36, kLeastShare = 24;
 // Tiles of all units up to which they are left to clusters: kFew where the clusters fill less than three quarters of the device, kMuch
 // otherwise.  A cluster's blocks take equal parts of one unit, so the longest unit sets the time; a line has a slower beginning and end.
-// Cluster and line, us, 4 kv heads of 128: 1 x 32000 tokens 16.8, 18.3; 4 x 32768 52, 32; 8 x 4000 12.8, 16.5, 8 of 10 to 4000 10.5, 12.5;
-// 8 x 16000 28.4, 32.1, 8 of 10 to 16000 26.4, 17.1; 36 x 4000 28.8, 30.4, 36 of 10 to 4000 25.0, 20.7.
+// Cluster and line, us, 4 kv heads of 128: 1 x 32000 tokens 16.8, 18.3; 4 x 32768 50.5, 32; 8 x 4000 12.8, 16.5, 8 of 10 to 4000 10.5,
+// 12.5; 8 x 16000 27.8, 31.8, 8 of 10 to 16000 26.4, 17.1; 36 x 4000 28.8, 30.4, 36 of 10 to 4000 25.0, 20.7.
 constexpr int kFew = 12288, kMuch = 24576;
 // Clusters of 1, 2, 4, 8 and 16 blocks that a device holds at once, per thousand SMs: blocks of kWarps (whose SMs hold several), and of
 // kWideWarps.  GPCs differ in their SMs, so it is not a matter of division (148 SMs: 592, 296, 142, 71 and 31; 148, 74, 33, 15 and 7).
@@ -270,7 +275,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
-  // Lengths and tables come as far as L2 while the kernel in front ends (a call from cold memory then has its first tile 0.7 us earlier);
+  // Lengths and tables come as far as L2 while the kernel in front ends (from cold memory 4 x 32768 tokens take 31.8 us for 32.2 without);
   // what they hold is read behind the wait.
   {
     const int at = int(blockIdx.x * kThreads + threadIdx.x), row = at / p.table_lines;

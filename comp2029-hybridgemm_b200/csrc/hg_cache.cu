@@ -1,7 +1,9 @@
 // A paged key-value cache held in MXFP8: quantising keys and values as they are written, and reading entries back.
 //
 // E4M3 codes with an E8M0 scale per 32 elements of a head, by the rule of hg_pack.  The layout is the one that
-// hg_attention.cu's loads ask for (see hg_cache.cuh).  Both are bound by memory, and in small calls by their chain: slot, entry.
+// hg_attention.cu's loads ask for (see hg_cache.cuh).  Both are bound by memory, and in small calls by their chain: slot, entry.  Eight
+// heads of 128, bf16, random slots: 65536 tokens written in 65 us and read in 73 (0.95 and 0.86 of the measured copy rate), 2048 in 3.9 and
+// 3.2 (0.50 and 0.61), 128 tokens of four heads in 1.3.
 #include <type_traits>
 
 #include "hg_cache.cuh"
@@ -12,7 +14,10 @@ namespace {
 // Eight threads to a token, head and key or value; each has four elements of every group of 32, whose 4 x GROUPS codes are consecutive in
 // the cache.  A block has kTokens tokens of one head.
 constexpr int kTokens = 8, kThreads = kTokens * 16;
-constexpr int kMany = 32768;   // tokens times heads from which a thread has two tokens
+// Tokens times heads from which a thread has two tokens: more loads are under way, but fewer SMs have some while there are few (one token
+// and two, us: 16384 x 8 heads written 19.5, 18.4, read 19.1, 14.5; 2048 x 8 written 3.9, 4.9, read 3.2, 3.6; at 4096 x 8 written 6.4, 6.6,
+// read 5.9, 4.8).
+constexpr int kMany = 32768;
 struct Place { uint8_t *codes, *scales; };   // of one thread's part of an entry
 template <int GROUPS>
 __device__ __forceinline__ Place place_of(const hg_cache& c, uint64_t by_page_size, uint32_t slot, int head, int kind, int x) {

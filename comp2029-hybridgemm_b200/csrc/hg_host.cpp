@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
@@ -300,7 +301,8 @@ PyObject* forward_epilogue(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // ---- calls between layers: None where an argument is not an ordinary one; Python then says what is wrong, or makes the call ----
 
 int64_t scale_bytes(int64_t rows, int64_t k) { return (rows + 127) / 128 * (k / 128) * 512; }
-at::Tensor bytes_like(const at::Tensor& t, at::IntArrayRef size) { return at::empty(size, at::TensorOptions().dtype(at::kByte).device(t.device())); }
+// A result on t's device, which is the current one.  Past the dispatcher a tensor costs 0.3 us less (a norm call with three 5.6 -> 4.9 us).
+at::Tensor result(at::IntArrayRef size, at::ScalarType type, const at::Tensor& t) { return at::Tensor(at::detail::empty_cuda(size, type, t.device(), std::nullopt)); }
 void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 bool failed(int status) {
   if (status) PyErr_SetString(PyExc_RuntimeError, last_error());
@@ -362,10 +364,10 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     {
       const Unlocked unlocked;
       const c10::cuda::CUDAGuard guard(x.device());
-      if (changed) stream = at::empty({rows, k}, x.options());
-      codes = packed ? bytes_like(x, {rows, k}) : at::empty({rows, k}, x.options());
+      if (changed) stream = result({rows, k}, x.scalar_type(), x);
+      codes = result({rows, k}, packed ? at::kByte : x.scalar_type(), x);
       if (packed) {
-        scales = bytes_like(x, {scale_bytes(rows, k)});
+        scales = result({scale_bytes(rows, k)}, at::kByte, x);
         call.codes = codes.mutable_data_ptr();
         call.scales = scales.mutable_data_ptr();
       } else {
@@ -450,9 +452,9 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
     {
       const Unlocked unlocked;
       const c10::cuda::CUDAGuard guard(data.device());
-      const auto options = at::TensorOptions().dtype(bf16 ? at::kBFloat16 : at::kHalf).device(data.device());
-      k = at::empty({slots.size(0), cache.kv_heads, head_dim}, options);
-      v = at::empty({slots.size(0), cache.kv_heads, head_dim}, options);
+      const auto type = bf16 ? at::kBFloat16 : at::kHalf;
+      k = result({slots.size(0), cache.kv_heads, head_dim}, type, data);
+      v = result({slots.size(0), cache.kv_heads, head_dim}, type, data);
       status = run_cache_read(&cache, k.mutable_data_ptr(), v.mutable_data_ptr(), static_cast<const int64_t*>(slots.const_data_ptr()), int(slots.size(0)),
                               bf16 ? HG_DTYPE_BF16 : HG_DTYPE_F16, stream_of(data));
     }
@@ -506,16 +508,16 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       status = bytes < 0 ? -1 : 0;
       if (!status) {
         if (packed) {
-          out = bytes_like(q, {seqs, heads * head_dim});
-          scales = bytes_like(q, {scale_bytes(seqs, heads * head_dim)});
+          out = result({seqs, heads * head_dim}, at::kByte, q);
+          scales = result({scale_bytes(seqs, heads * head_dim)}, at::kByte, q);
           call.codes = out.mutable_data_ptr();
           call.scales = scales.mutable_data_ptr();
         } else {
-          out = at::empty({seqs, heads, head_dim}, q.options());
+          out = result({seqs, heads, head_dim}, q.scalar_type(), q);
           call.out = out.mutable_data_ptr();
         }
         if (with_lse) {
-          lse = at::empty({seqs, heads}, q.options().dtype(at::kFloat));
+          lse = result({seqs, heads}, at::kFloat, q);
           call.lse = static_cast<float*>(lse.mutable_data_ptr());
         }
         if (bytes) workspace = c10::cuda::CUDACachingAllocator::get()->allocate(size_t(bytes));
