@@ -16,7 +16,7 @@
 //
 // What bounds it: bytes of the cache, and nearly as soon a warp's way through a tile (about 435 instructions for 4224 bytes, issued in half
 // of the slots, with the ALU pipe busy as long; from L2 an SM keeps up with some 24 bytes a clock, and memory delivers 23.6).  28 heads on 4 of 128, bf16: 128 sequences of 1024 to 1150 tokens
-// 31.7 us (0.72 of the measured copy rate), 128 x 4000 about 94 us (0.88), 4 x 32768 32.0 us (0.66); 1 x 1000 5.2 us, of which launch, three
+// 31.7 us (0.72 of the measured copy rate), 128 x 4000 about 94 us (0.88), 4 x 32768 30.3 us (0.70); 1 x 1000 5.2 us, of which launch, three
 // dependent loads and two meetings of blocks are all but 0.2.
 //
 // Roundings: q keeps its 16 bits (a head's bf16 queries become halves under a power of two, which keeps eight bits of all that is
@@ -24,7 +24,7 @@
 // between 2^-32 and 2^8 of the largest so far by a bias of 2^7 and lazy rescaling.  Sums, maxima and outputs are fp32.  Where the output
 // is quantised (EXACT) what the rounding of P left goes through a second product: an output beside the border of two scales changes the codes
 // of its whole group, and a rounding to 16 bits no longer hides the difference.  (37 sequences, codes against 64-bit arithmetic:
-// relative difference 0.015 with one product, none with two, 0.010 in fp32 arithmetic; 17.9 us and 18.3.)
+// relative difference 0.015 with one product, none with two, 0.010 in fp32 arithmetic; 17.0 us and 17.4.)
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -44,14 +44,17 @@ constexpr int kWarps = 4, kWideWarps = 12;   // of a block; of one that has an S
 constexpr int kMostRing = 4;        // tiles of a warp in shared memory or on their way there, at most
 constexpr int kBlocksPerSm = 4, kLineBlocksPerSm = 3;   // of kWarps; of a line of no more units than that
 constexpr int kWhole = 16;           // sequences of no more tiles are not split
-// Costs in tiles.  A unit costs kUnitCost beside its tiles, units that are split kSplitCost (in a block of kWarps), and a block takes at
-// least kLeastShare.
-constexpr int kUnitCost = 16, kSplitCost = 36, kLeastShare = 24;
+// Costs in tiles.  A unit has one beside its tiles, by the warps that share these (16 for both: 37 of 1 to 4099 tokens on three blocks an SM 17.4
+// us for 17.05, 16 of 10 to 16000 on wide ones 19.3 for 17.4), units that are split have kSplitCost (in a block of kWarps), and a block takes at
+// least kLeastShare (40: 37 of 1 to 4099 18.4 us).
+constexpr int kSplitCost = 36, kLeastShare = 24;
+__host__ __device__ constexpr int unit_cost(int warps) { return warps == kWarps ? 12 : 24; }
 // Tiles of all units up to which they are left to clusters: kFew where the clusters fill less than three quarters of the device, kMuch
 // otherwise.  A cluster's blocks take equal parts of one unit, so the longest unit sets the time; a line has a slower beginning and end.
-// Cluster and line, us, 4 kv heads of 128: 1 x 32000 tokens 16.8, 18.3; 4 x 32768 50.5, 32; 8 x 4000 12.8, 16.5, 8 of 10 to 4000 10.5,
-// 12.5; 8 x 16000 27.8, 31.8, 8 of 10 to 16000 26.4, 17.1; 36 x 4000 28.8, 30.4, 36 of 10 to 4000 25.0, 20.7.
-constexpr int kFew = 12288, kMuch = 24576;
+// Cluster and line, us, 4 kv heads of 128: 1 x 8000 tokens 8.3, 11.1; 1 x 32000 16.6, 16.7; 4 x 4000 12.1, 12.6; 4 x 16000 28.1, 19.4; 4 x 32768 50.5,
+// 30.3; 8 x 4000 12.8, 15.0, 8 of 10 to 4000 10.3, 10.4; 8 x 16000 27.8, 29.7, 8 of 10 to 16000 26.4, 14.6; 16 x 2000 13.1, 16.2, 16 of 10 to
+// 2000 8.8, 10.4; 36 x 4000 28.8, 28.6, 36 of 10 to 4000 25.0, 15.9.
+constexpr int kFew = 6144, kMuch = 18432;
 // Clusters of 1, 2, 4, 8 and 16 blocks that a device holds at once, per thousand SMs: blocks of kWarps (whose SMs hold several), and of
 // kWideWarps.  GPCs differ in their SMs, so it is not a matter of division (148 SMs: 592, 296, 142, 71 and 31; 148, 74, 33, 15 and 7).
 constexpr int kHeld[2][5] = {{4000, 2000, 959, 479, 209}, {1000, 500, 222, 101, 47}};
@@ -61,7 +64,7 @@ constexpr float kNone = -3e38f;      // maximum of nothing
 constexpr int kLeastScale = 24;      // values are summed under 2^-103 at least
 
 // How units come to blocks.  Few units (CLUSTER): a cluster of `split` blocks each, whose sums meet in shared memory.  Many (LINE):
-// the work is a line on which every unit (sequence and head unit, in this order) has its tiles behind kUnitCost for what it costs
+// the work is a line on which every unit (sequence and head unit, in this order) has its tiles behind what it costs
 // besides, and a block takes an equal share of it, so whatever the lengths all blocks end together.  A unit that ends in another
 // block than it begins in is added up by the one that it begins in, which comes to it last; the others come to their
 // parts of it first, write their sums to a slot and set a tag behind them, and the first one waits for the tags and takes them back.
@@ -235,14 +238,21 @@ __device__ __forceinline__ bool wait_for(const uint64_t* at, uint64_t tag) {
   }
 }
 
+// Whether sums have a place of their own on a line, so that the next unit's first tiles and queries come in while one's are added up: where three
+// tiles to a warp are left beside them (4 x 32768 tokens 31.9 -> 30.3 us, 16 of 10 to 16000 22.6 -> 19.3, 37 of 1 to 4099 18.0 -> 17.4, 64 x 500 14.65 ->
+// 14.1).
+__host__ __device__ constexpr bool apart(int head_dim, int per_sm) { return head_dim == 64 || per_sm < kBlocksPerSm; }
+
 // Shared memory of a block.  A tile of keys or values is 16 rows of head_dim bytes, whose 16-byte chunks the copy swizzles (with the
-// period of 128-byte rows, or of 64-byte ones).  The warps' sums take the place of the rings when these are idle.
+// period of 128-byte rows, or of 64-byte ones).  The warps' sums take the place of the rings when these are idle, or (apart)
+// have their own, so that the next unit's first tiles come in meanwhile.
 template <int GROUPS, int WARPS>
 struct Shared {
   static constexpr int kDim = 32 * GROUPS, kCodes = kTile * kDim, kScales = kTile * 2 * GROUPS, kRow = kDim + 4;
   static constexpr int kStage = 2 * kCodes + kScales;   // of a warp
-  static int bytes(int ring) {
-    return std::max(WARPS * ring * kStage, WARPS * kHeadTile * kRow * 4) + 1024;   // the beginning is brought to a multiple of 1024
+  static constexpr int kSums = WARPS * kHeadTile * kRow * 4;
+  static constexpr int bytes(int ring, bool apart) {
+    return (apart ? WARPS * ring * kStage + kSums : (WARPS * ring * kStage > kSums ? WARPS * ring * kStage : kSums)) + 1024;   // the beginning is brought to a multiple of 1024
   }
 };
 // Row r of a fragment's eight holds this token: two rows that are read in one pass, r and r ^ 1, then have their chunks in different
@@ -259,6 +269,8 @@ __global__ void __launch_bounds__(WARPS * 32, PER_SM)
 attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ CUtensorMap map) {
   using S = Shared<GROUPS, WARPS>;
   constexpr int kDim = 32 * GROUPS, kThreads = WARPS * 32;
+  constexpr int kUnitCost = unit_cost(WARPS);
+  constexpr bool kApart = LINE && apart(kDim, PER_SM);
   extern __shared__ uint8_t dynamic[];
   __shared__ int given_up, there[WARPS][kMostRing];
   __shared__ float weights[WARPS][kHeadTile], maxima[WARPS][kHeadTile];
@@ -267,7 +279,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int ring = p.ring;
   const uint32_t base = (smem_u32(dynamic) + 1023u) & ~1023u, all_scales = base + uint32_t(WARPS * ring) * (2 * S::kCodes), bars = smem_u32(&full[warp][0]);
-  float (*const sums)[kHeadTile][S::kRow] = reinterpret_cast<float (*)[kHeadTile][S::kRow]>(dynamic + (base - smem_u32(dynamic)));
+  float (*const sums)[kHeadTile][S::kRow] = reinterpret_cast<float (*)[kHeadTile][S::kRow]>(dynamic + (base - smem_u32(dynamic)) + (kApart ? WARPS * ring * S::kStage : 0));
   if (lane < p.ring) mbar_init(bars + 8 * lane, 1);
   if (threadIdx.x == 0) {
     given_up = 0;
@@ -275,7 +287,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
-  // Lengths and tables come as far as L2 while the kernel in front ends (from cold memory 4 x 32768 tokens take 31.8 us for 32.2 without);
+  // Lengths and tables come as far as L2 while the kernel in front ends (from cold memory 4 x 32768 tokens took 31.8 us for 32.2 without);
   // what they hold is read behind the wait.
   {
     const int at = int(blockIdx.x * kThreads + threadIdx.x), row = at / p.table_lines;
@@ -324,7 +336,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     largest += kUnitCost;
     share = max(int64_t(kLeastShare), int64_t(float(s.all) * p.by_blocks) + 1);   // at least s.all / blocks
     // No unit is split where the longest of them, as many as a block gets, cost no more than an equal share and a split.  Whole and split, us:
-    // 64 x 500 tokens of 4 heads 14.8, 18.9, 64 x 2000 39.9, 35.1; 40 x 4000 72, 38; 96 x 4000 75.1, 77.5; 128 x 2000 53.2, 57.2.
+    // 64 x 500 tokens of 4 heads 14.1, 17.9, 64 x 2000 39.9, 33.0; 40 x 4000 72, 37; 96 x 2000 39.1, 43.7.
     whole = int64_t(largest) * (p.least + (p.more > 0)) <= share + kSplitCost * WARPS / kWarps;
     if (whole) {
       // blocks with one unit more are spread over the SMs
@@ -370,13 +382,18 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   const uint32_t key_at = chunk_at<GROUPS>(my_token, c);
   const uint32_t value_at = GROUPS == 4 ? chunk_at<4>(value_token, r) : chunk_at<2>(value_token, r >> 1) + 8 * (r & 1);
   const uint32_t odd_at = GROUPS == 4 ? chunk_at<4>(odd_token, r) : chunk_at<2>(odd_token, r >> 1) + 8 * (r & 1);
-  while (remaining > 0) {
+  // The unit at `position`: its tiles, heads and, on the line, the part of its cost that falls to this block.
+  Span span;
+  int begin, end, from = 0, to = 0, cost = 0, kv_head, head0, heads;
+  const int* table;
+  // Copies run ahead of the tiles that are multiplied.  The number of the next tile's page is on its way a tile earlier.
+  int ahead_tile, ahead_page;
+  auto enter = [&] {
     if (whole) {
       seq = int(position) / p.head_units;
       head_unit = int(position) - seq * p.head_units;
     }
-    const Span span = span_of(p, seq);
-    int begin, end, from = 0, to = 0, cost = 0;   // tiles; the part of the unit's cost
+    span = span_of(p, seq);
     if (!whole) {
       cost = span.to - span.from + kUnitCost;
       head_unit = int(uint32_t(offset) / uint32_t(cost));
@@ -392,52 +409,70 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       begin = min(span.to, span.from + rank * tiles);
       end = min(span.to, begin + tiles);
     }
-    const int kv_head = head_unit / p.chunks, chunk = head_unit - kv_head * p.chunks;
-    const int head0 = kv_head * p.group + chunk * kHeadTile, heads = min(kHeadTile, p.group - chunk * kHeadTile);
-
-    // Copies run ahead of the tiles that are multiplied.  The number of the next tile's page is on its way a tile earlier.
-    const int* const table = p.call.table + seq * p.call.table_stride;
-    int ahead_tile = begin + warp, ahead_page = ahead_tile < end ? table[place_of(ahead_tile)] : 0;
-    auto copy_next = [&] {
-      if (ahead_tile >= end) return;
-      const int next_page = ahead_tile + WARPS < end ? table[place_of(ahead_tile + WARPS)] : 0;
-      if (elect_one()) {
-        // A page that is not there gives way to the first one, whose entries are then not used.
-        const bool here = uint32_t(ahead_page) < uint32_t(p.cache.pages);
-        const int record = (here ? ahead_page : 0) * p.cache.kv_heads + kv_head;
-        const int entry = (ahead_tile - place_of(ahead_tile) * int(p.page_tiles)) * kTile, row = record * record_rows + entry;
-        const uint32_t bar = bars + 8 * copied, slot = uint32_t(warp * ring + copied);
-        there[warp][copied] = here;
-        mbar_expect_tx(bar, 2 * S::kCodes + S::kScales);
-        tma_load_2d(base + slot * (2 * S::kCodes), &map, bar, 0, row);
-        tma_load_2d(base + slot * (2 * S::kCodes) + S::kCodes, &map, bar, 0, row + p.cache.page_size);
-        bulk_load(all_scales + slot * S::kScales,
-                  static_cast<const uint8_t*>(p.cache.data) + (int64_t(record) * record_rows + 2 * p.cache.page_size) * kDim + entry * 2 * GROUPS, S::kScales, bar);
-      }
-      __syncwarp();
-      copied = copied == ring - 1 ? 0 : copied + 1;
-      ahead_tile += WARPS;
-      ahead_page = next_page;
-    };
+    kv_head = head_unit / p.chunks;
+    const int chunk = head_unit - kv_head * p.chunks;
+    head0 = kv_head * p.group + chunk * kHeadTile;
+    heads = min(kHeadTile, p.group - chunk * kHeadTile);
+    table = p.call.table + seq * p.call.table_stride;
+    ahead_tile = begin + warp;
+    ahead_page = ahead_tile < end ? table[place_of(ahead_tile)] : 0;
+  };
+  auto copy_next = [&] {
+    if (ahead_tile >= end) return;
+    const int next_page = ahead_tile + WARPS < end ? table[place_of(ahead_tile + WARPS)] : 0;
+    if (elect_one()) {
+      // A page that is not there gives way to the first one, whose entries are then not used.
+      const bool here = uint32_t(ahead_page) < uint32_t(p.cache.pages);
+      const int record = (here ? ahead_page : 0) * p.cache.kv_heads + kv_head;
+      const int entry = (ahead_tile - place_of(ahead_tile) * int(p.page_tiles)) * kTile, row = record * record_rows + entry;
+      const uint32_t bar = bars + 8 * copied, slot = uint32_t(warp * ring + copied);
+      there[warp][copied] = here;
+      mbar_expect_tx(bar, 2 * S::kCodes + S::kScales);
+      tma_load_2d(base + slot * (2 * S::kCodes), &map, bar, 0, row);
+      tma_load_2d(base + slot * (2 * S::kCodes) + S::kCodes, &map, bar, 0, row + p.cache.page_size);
+      bulk_load(all_scales + slot * S::kScales,
+                static_cast<const uint8_t*>(p.cache.data) + (int64_t(record) * record_rows + 2 * p.cache.page_size) * kDim + entry * 2 * GROUPS, S::kScales, bar);
+    }
+    __syncwarp();
+    copied = copied == ring - 1 ? 0 : copied + 1;
+    ahead_tile += WARPS;
+    ahead_page = next_page;
+  };
+  uint32_t q[GROUPS][2][2];
+  auto fetch = [&] {   // the unit's first tiles and queries
 #pragma unroll 1
     for (int i = 0; i < ring - 1 && !lost; ++i) copy_next();
-
+    const uint16_t* const row = static_cast<const uint16_t*>(p.call.q) + seq * p.call.q_stride + int64_t(head0 + r) * kDim;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        const int x = GROUPS == 4 ? 4 * j + c : 2 * c + j;
+        const uint2 v = r < heads ? *reinterpret_cast<const uint2*>(row + 32 * g + 4 * x) : make_uint2(0, 0);
+        q[g][j][0] = v.x;
+        q[g][j][1] = v.y;
+      }
+  };
+  if constexpr (kApart) {
+    enter();
+    fetch();
+  }
+  for (;;) {
+    if constexpr (!kApart) {
+      enter();
+      fetch();
+    }
     // Queries as the second operand of the first product: column r is head r, rows the four elements at 32 g + 4 x.  A head's bf16 queries
     // become halves under a power of two that brings the largest to [2^14, 2^15).
-    uint32_t q[GROUPS][2][2];
     float2 to_log2;
     {
-      const uint16_t* const row = static_cast<const uint16_t*>(p.call.q) + seq * p.call.q_stride + int64_t(head0 + r) * kDim;
       uint32_t top = 0;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
-          const int x = GROUPS == 4 ? 4 * j + c : 2 * c + j;
-          const uint2 v = r < heads ? *reinterpret_cast<const uint2*>(row + 32 * g + 4 * x) : make_uint2(0, 0);
-          q[g][j][0] = v.x;
-          q[g][j][1] = v.y;
-          top = max(max(top, max(v.x & 0x7fffu, (v.x >> 16) & 0x7fffu)), max(v.y & 0x7fffu, (v.y >> 16) & 0x7fffu));
+          const uint32_t v0 = q[g][j][0], v1 = q[g][j][1];
+          top = max(max(top, max(v0 & 0x7fffu, (v0 >> 16) & 0x7fffu)), max(v1 & 0x7fffu, (v1 >> 16) & 0x7fffu));
         }
       float back = p.call.scale * 1.44269504f;
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
@@ -643,8 +678,40 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       }
     }
 
+    // On to the next unit, whose first tiles come in while this one's sums are added up where these are apart.
+    const bool begins = from == 0, ends = to == cost;   // whole units: both
+    const int done_seq = seq, done_head0 = head0, done_heads = heads;
+    int others = 0;   // where the unit ends in a block behind this one, this block waits for the parts of the blocks up to there
+    auto find_others = [&] {
+      if (!begins || ends) return;
+      const int64_t last = position + cost - 1 - blockIdx.x * share;   // of the unit, behind this block's first place
+      others = share >> 31 ? int(last >= share) : int(uint32_t(last) / uint32_t(share));
+    };
+    auto advance = [&] {
+      if (whole) {
+        --remaining;
+        ++position;
+      } else {
+        remaining -= to - from;
+        offset += to - from;
+        position += to - from;
+        if (offset == cost * p.head_units) {
+          ++seq;
+          offset = 0;
+        }
+      }
+    };
+    if constexpr (kApart) {
+      find_others();
+      advance();
+      if (remaining > 0) {
+        enter();
+        fetch();
+      }
+    }
+
     // The block's warps meet: sums under a common maximum.
-    __syncthreads();   // the rings are idle
+    __syncthreads();   // the rings are idle, and sums that were there have been read
     const float unit_scale = lost ? __uint_as_float(0x7fc00000u) : mx_scale(value_scale);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -662,19 +729,13 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
         *reinterpret_cast<float4*>(&sums[warp][2 * c + h][32 * g + 4 * r]) =
             make_float4(out[g][0][h] * unit_scale, out[g][0][h + 2] * unit_scale, out[g][1][h] * unit_scale, out[g][1][h + 2] * unit_scale);
     __syncthreads();
-    const bool begins = from == 0, ends = to == cost;   // whole units: both
-    // Where the unit ends in a block behind this one, this block waits for the parts of the blocks up to there.
-    int others = 0;
-    if (LINE && begins && !ends) {
-      const int64_t last = position + cost - 1 - blockIdx.x * share;   // of the unit, behind this block's first place
-      others = share >> 31 ? int(last >= share) : int(uint32_t(last) / uint32_t(share));
-    }
+    if constexpr (LINE && !kApart) find_others();
     if (others) {
       for (int i = threadIdx.x; i < others; i += kThreads)
         if (!wait_for(p.tags + blockIdx.x + 1 + i, p.tag)) given_up = 1;
       __syncthreads();
     }
-    for (int i = threadIdx.x; i < heads * kDim / 4; i += kThreads) {   // whole groups of eight lanes
+    for (int i = threadIdx.x; i < done_heads * kDim / 4; i += kThreads) {   // whole groups of eight lanes
       const int h = i / (kDim / 4), d = (i % (kDim / 4)) * 4;
       float m = maxima[0][h], l = 0.f;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -701,9 +762,9 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
           y = __ldcg(reinterpret_cast<const float2*>(partial + j * kStride + kHeadTile * kDim + 2 * h));
         });
         if (others && given_up) l = __uint_as_float(0x7fc00000u);
-        write_out<T, GROUPS>(p, seq, head0 + h, d, sum, l, m);
+        write_out<T, GROUPS>(p, done_seq, done_head0 + h, d, sum, l, m);
       } else if (p.split == 1) {
-        write_out<T, GROUPS>(p, seq, head0 + h, d, sum, l, m);
+        write_out<T, GROUPS>(p, done_seq, done_head0 + h, d, sum, l, m);
       } else {
         *reinterpret_cast<float4*>(&sums[0][h][d]) = sum;   // read by this thread alone until here
         if (d == 0) block_weights[h] = make_float2(m, l);
@@ -716,29 +777,18 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       } else if (others) {
         for (int i = threadIdx.x; i < others; i += kThreads) p.tags[blockIdx.x + 1 + i] = 0;
       }
-      if (whole) {
-        --remaining;
-        ++position;
-      } else {
-        remaining -= to - from;
-        offset += to - from;
-        position += to - from;
-        if (offset == cost * p.head_units) {
-          ++seq;
-          offset = 0;
-        }
-      }
-      if (remaining > 0) {   // the sums have been read, and copies may take their place
+      if constexpr (!kApart) advance();
+      if (remaining <= 0) break;
+      if constexpr (!kApart) {   // the sums have been read, and copies may take their place
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
       }
     } else {
-      remaining = 0;
       if (p.split > 1) {
         // The cluster's blocks meet: each adds up its share of the columns over all blocks, in their order.
         cluster_sync();
         const int columns = kHeadTile * kDim / 4 / p.split, i = rank * columns + threadIdx.x;   // at least two blocks, 128 threads
-        if (threadIdx.x < columns && i < heads * kDim / 4) {   // whole groups of eight lanes
+        if (threadIdx.x < columns && i < done_heads * kDim / 4) {   // whole groups of eight lanes
           const int h = i / (kDim / 4), d = (i % (kDim / 4)) * 4;
           const uint32_t sums_at = smem_u32(&sums[0][h][d]), weights_at = smem_u32(&block_weights[h]);
           float m = kNone, l = 0.f;
@@ -747,10 +797,11 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
             asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(map_to_rank(sums_at, uint32_t(j))) : "memory");
             asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(y.x), "=f"(y.y) : "r"(map_to_rank(weights_at, uint32_t(j))) : "memory");
           });
-          write_out<T, GROUPS>(p, seq, head0 + h, d, sum, l, m);
+          write_out<T, GROUPS>(p, done_seq, done_head0 + h, d, sum, l, m);
         }
         cluster_sync();   // no block leaves while another may read its sums
       }
+      break;
     }
   }
   if (lost) {   // time for what is still on its way to shared memory
@@ -791,15 +842,17 @@ Split split_of(const hg_cache& c, int seqs, int heads, int table_width, int wind
   if (s.line) {
     // Few units have many parts each: a wide block to an SM makes these a third as many, and its warps end together (4 x 32768: 31.9 us; three
     // blocks 34.5).  With more units, blocks that begin and end one at different times cover for one another (37 of 1 to 4099: 18.3;
-    // one wide block 26.1).
+    // one wide block 26.1).  Four blocks an SM have no room for sums beside rings of 128 elements (see kApart): they take what gives each of them
+    // one unit at most (128 x 1100 31.7 us, three blocks 36.4; 128 of 10 to 3000 tokens of 8 heads 38.7, 37.7).
     const bool wide = s.units <= sms;
     s.warps = wide ? kWideWarps : kWarps;
-    s.per_sm = wide ? 1 : s.units <= sms * kLineBlocksPerSm ? kLineBlocksPerSm : kBlocksPerSm;
+    s.per_sm = wide ? 1 : s.units <= sms * kLineBlocksPerSm || (s.units > sms * kBlocksPerSm && c.head_dim == 128) ? kLineBlocksPerSm : kBlocksPerSm;
     s.split = 1;
-    s.blocks = int(std::min<int64_t>(sms * s.per_sm, (s.units * (longest + kUnitCost) + kLeastShare - 1) / kLeastShare));
+    s.blocks = int(std::min<int64_t>(sms * s.per_sm, (s.units * (longest + unit_cost(s.warps)) + kLeastShare - 1) / kLeastShare));
   }
   // As deep a ring as the blocks of an SM have room for, and use.
-  const int room = (kSmBytes / s.per_sm - 2048) / (s.warps * (c.head_dim == 128 ? Shared<4, kWarps>::kStage : Shared<2, kWarps>::kStage));
+  const int sums = s.line && apart(c.head_dim, s.per_sm) ? s.warps * kHeadTile * (c.head_dim + 4) * 4 : 0;
+  const int room = (kSmBytes / s.per_sm - 2048 - sums) / (s.warps * (c.head_dim == 128 ? Shared<4, kWarps>::kStage : Shared<2, kWarps>::kStage));
   s.ring = std::max(2, std::min({kMostRing, room, int((longest / s.split + s.warps - 1) / s.warps) + 1}));
   return s;
 }
@@ -811,7 +864,7 @@ void validate_attention(const hg_cache& c, int seqs, int heads, int table_width,
   if (seqs < 0 || heads <= 0 || heads % c.kv_heads) throw std::runtime_error("hg_attention: heads must be a multiple of kv_heads");
   if (table_width < 0 || window < 0 || int64_t(table_width) * c.page_size > (int64_t(1) << 30)) throw std::runtime_error("hg_attention: invalid table width or window");
   // a sequence's units are counted in 32 bits
-  if (int64_t(seqs) * heads > (1 << 26) || (int64_t(table_width) * c.page_size / kTile + kUnitCost + 1) * heads > 0x7fffffff) throw std::runtime_error("hg_attention: too much work for one call");
+  if (int64_t(seqs) * heads > (1 << 26) || (int64_t(table_width) * c.page_size / kTile + unit_cost(kWideWarps) + 1) * heads > 0x7fffffff) throw std::runtime_error("hg_attention: too much work for one call");
 }
 
 // The cache as rows of head_dim bytes; a copy takes sixteen.
@@ -831,13 +884,16 @@ CUtensorMap cache_map(const hg_cache& c) {
 
 template <typename T, int GROUPS, int WARPS, int PER_SM, bool LINE, bool EXACT>
 void launch_attention(const AttentionParams& p, const Split& s, cudaStream_t stream) {
-  const int bytes = Shared<GROUPS, WARPS>::bytes(s.ring);
+  constexpr bool kApart = LINE && apart(32 * GROUPS, PER_SM);
+  constexpr int kMost = Shared<GROUPS, WARPS>::bytes(kApart && GROUPS == 4 ? 3 : kMostRing, kApart);
+  const int bytes = Shared<GROUPS, WARPS>::bytes(s.ring, kApart);
+  if (bytes > kMost) throw std::runtime_error("hg_attention: shared memory");
   static std::once_flag once[64];   // limits of the function on each device
   int device = 0;
   check(cudaGetDevice(&device), "cudaGetDevice");
   if (device < 0 || device >= 64) throw std::runtime_error("Device ordinals 0..63 are supported");
   std::call_once(once[device], [] {
-    check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, WARPS, PER_SM, LINE, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shared<GROUPS, WARPS>::bytes(kMostRing)), "attention");
+    check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, WARPS, PER_SM, LINE, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost), "attention");
     check(cudaFuncSetAttribute(attention_kernel<T, GROUPS, WARPS, PER_SM, LINE, EXACT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "attention");
   });
   cudaLaunchConfig_t config{};

@@ -123,6 +123,7 @@ class PagedCache:
         sequence that sees nothing (length 0) gives zeros and minus infinity.  A length beyond the table is cut to it, and the
         positions of a page number outside the cache (-1, say, where a page was given up) are left out.  What the table holds
         behind a sequence's last page, and the cache behind its last position, has no influence, NaNs included.
+        How the work is spread over the device is chosen by the table's width, so a table far wider than its sequences costs a few us.
         """
         return self._attend(q, page_table, lengths, scale, window, lse, False)
 
