@@ -24,7 +24,7 @@
 // between 2^-32 and 2^8 of the largest so far by a bias of 2^7 and lazy rescaling.  Sums, maxima and outputs are fp32.  Where the output
 // is quantised (EXACT) what the rounding of P left goes through a second product: an output beside the border of two scales changes the codes
 // of its whole group, and a rounding to 16 bits no longer hides the difference.  (37 sequences, codes against 64-bit arithmetic:
-// relative difference 0.015 with one product, none with two, 0.010 in fp32 arithmetic; 17.0 us and 17.4.)
+// relative difference 0.015 with one product, none with two, 0.010 in fp32 arithmetic; 16.6 us and 17.0.)
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -45,9 +45,9 @@ constexpr int kMostRing = 4;        // tiles of a warp in shared memory or on th
 constexpr int kBlocksPerSm = 4, kLineBlocksPerSm = 3;   // of kWarps; of a line of no more units than that
 constexpr int kWhole = 16;           // sequences of no more tiles are not split
 // Costs in tiles.  A unit has one beside its tiles, by the warps that share these (16 for both: 37 of 1 to 4099 tokens on three blocks an SM 17.4
-// us for 17.05, 16 of 10 to 16000 on wide ones 19.3 for 17.4), units that are split have kSplitCost (in a block of kWarps), and a block takes at
+// us for 17.05; 16 of 10 to 16000 on wide ones 19.3 for 17.4), units that are split have kSplitCost (in a block of kWarps), and a block takes at
 // least kLeastShare (40: 37 of 1 to 4099 18.4 us).
-constexpr int kSplitCost = 36, kLeastShare = 24;
+constexpr int kSplitCost = 28, kLeastShare = 24;
 __host__ __device__ constexpr int unit_cost(int warps) { return warps == kWarps ? 12 : 24; }
 // Tiles of all units up to which they are left to clusters: kFew where the clusters fill less than three quarters of the device, kMuch
 // otherwise.  A cluster's blocks take equal parts of one unit, so the longest unit sets the time; a line has a slower beginning and end.
@@ -336,7 +336,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     largest += kUnitCost;
     share = max(int64_t(kLeastShare), int64_t(float(s.all) * p.by_blocks) + 1);   // at least s.all / blocks
     // No unit is split where the longest of them, as many as a block gets, cost no more than an equal share and a split.  Whole and split, us:
-    // 64 x 500 tokens of 4 heads 14.1, 17.9, 64 x 2000 39.9, 33.0; 40 x 4000 72, 37; 96 x 2000 39.1, 43.7.
+    // 64 x 700 tokens of 4 heads 17.3, 18.5, 64 x 1000 22.2, 21.4, 64 x 2000 39.9, 31.4; 40 x 4000 72, 37; 96 x 2000 39.1, 43.7.
     whole = int64_t(largest) * (p.least + (p.more > 0)) <= share + kSplitCost * WARPS / kWarps;
     if (whole) {
       // blocks with one unit more are spread over the SMs
@@ -757,10 +757,13 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
           continue;
         }
         const float* const partial = p.partial + (blockIdx.x + 1) * kStride;
-        meet<16>(others, m, l, sum, [&](int j, float4& x, float2& y) {
+        const auto load = [&](int j, float4& x, float2& y) {
           x = __ldcg(reinterpret_cast<const float4*>(partial + j * kStride + h * kDim + d));
           y = __ldcg(reinterpret_cast<const float2*>(partial + j * kStride + kHeadTile * kDim + 2 * h));
-        });
+        };
+        // Few together where there are few: with sixteen at a time, most of them read again, 128 of 1000 to 2000 tokens took 44.4 us for 42.5.
+        if (others <= 4) meet<2>(others, m, l, sum, load);
+        else meet<16>(others, m, l, sum, load);
         if (others && given_up) l = __uint_as_float(0x7fc00000u);
         write_out<T, GROUPS>(p, done_seq, done_head0 + h, d, sum, l, m);
       } else if (p.split == 1) {
@@ -793,10 +796,13 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
           const uint32_t sums_at = smem_u32(&sums[0][h][d]), weights_at = smem_u32(&block_weights[h]);
           float m = kNone, l = 0.f;
           float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-          meet<8>(p.split, m, l, sum, [&](int j, float4& x, float2& y) {
+          const auto load = [&](int j, float4& x, float2& y) {
             asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(map_to_rank(sums_at, uint32_t(j))) : "memory");
             asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(y.x), "=f"(y.y) : "r"(map_to_rank(weights_at, uint32_t(j))) : "memory");
-          });
+          };
+          if (p.split == 2) meet<2>(2, m, l, sum, load);
+          else if (p.split == 4) meet<4>(4, m, l, sum, load);
+          else meet<8>(p.split, m, l, sum, load);
           write_out<T, GROUPS>(p, done_seq, done_head0 + h, d, sum, l, m);
         }
         cluster_sync();   // no block leaves while another may read its sums
@@ -843,7 +849,7 @@ Split split_of(const hg_cache& c, int seqs, int heads, int table_width, int wind
     // Few units have many parts each: a wide block to an SM makes these a third as many, and its warps end together (4 x 32768: 31.9 us; three
     // blocks 34.5).  With more units, blocks that begin and end one at different times cover for one another (37 of 1 to 4099: 18.3;
     // one wide block 26.1).  Four blocks an SM have no room for sums beside rings of 128 elements (see kApart): they take what gives each of them
-    // one unit at most (128 x 1100 31.7 us, three blocks 36.4; 128 of 10 to 3000 tokens of 8 heads 38.7, 37.7).
+    // one unit at most (128 x 1100 31.7 us, three blocks 34.1; 128 of 1000 to 2000 42.5, 41.2).
     const bool wide = s.units <= sms;
     s.warps = wide ? kWideWarps : kWarps;
     s.per_sm = wide ? 1 : s.units <= sms * kLineBlocksPerSm || (s.units > sms * kBlocksPerSm && c.head_dim == 128) ? kLineBlocksPerSm : kBlocksPerSm;
