@@ -139,7 +139,9 @@ def test_many_entries(dtype):
 @pytest.mark.parametrize("case", [
     (768, 3584, torch.bfloat16, True, None, 1.0, False), (771, 1024, torch.float16, True, "channel", 1.0, True),
     (800, 1152, torch.float16, True, "token", 0.5, False), (1025, 8320, torch.bfloat16, False, "element", 1.0, True),
-    (769, 18944, torch.bfloat16, True, None, 1.0, False)], ids=lambda c: f"{c[0]}x{c[1]}")
+    (769, 18944, torch.bfloat16, True, None, 1.0, False), (1153, 8192, torch.bfloat16, True, "channel", 1.0, True),
+    (770, 12288, torch.float16, True, None, 1.0, False), (1400, 7168, torch.bfloat16, False, "token", 2.0, False),
+    (600, 16384, torch.bfloat16, True, "element", 1.0, True), (1600, 7296, torch.float16, False, None, 1.0, False)], ids=lambda c: f"{c[0]}x{c[1]}")
 def test_norm_of_many_rows(case):
     operands = inputs(*case)
     q, sf, h = producer.norm_pack(eps=1e-6, **operands)
