@@ -58,6 +58,7 @@ constexpr int kFew = 6144, kMuch = 18432;
 // Clusters of 1, 2, 4, 8 and 16 blocks that a device holds at once, per thousand SMs: blocks of kWarps (whose SMs hold several), and of
 // kWideWarps.  GPCs differ in their SMs, so it is not a matter of division (148 SMs: 592, 296, 142, 71 and 31; 148, 74, 33, 15 and 7).
 constexpr int kHeld[2][5] = {{4000, 2000, 959, 479, 209}, {1000, 500, 222, 101, 47}};
+constexpr int kTableLines = 8192;    // lines of the table that are prefetched, at most: it may be far wider than its sequences
 constexpr int kSmBytes = 228 << 10;  // shared memory of an SM
 constexpr float kBias = 7.f, kSlack = 4.f;   // P is kept in [0, 2^(kBias + 2 kSlack)]
 constexpr float kNone = -3e38f;      // maximum of nothing
@@ -82,7 +83,7 @@ struct AttentionParams {
   uint64_t tag;
   int least, more;      // LINE: units of a block, and blocks that have one more
   float by_blocks;      // LINE: 1 / blocks, rounded up
-  int table_lines;      // 128-byte lines of a row of the table
+  int table_lines;      // 128-byte lines of a row of the table that are prefetched
   int head_units;       // kv heads x chunks of kHeadTile heads
   int chunks, group;
   int split;            // CLUSTER: blocks of a unit, 1, 2, 4, 8 or 16
@@ -954,7 +955,7 @@ int hg_attention(const hg_cache* cache, const hg_attention_call* call, int dtype
     throw std::runtime_error("hg_attention: pointers must be aligned to 16 bytes and q_stride to 8 elements");
   const hg::Split s = hg::split_of(*cache, a.seqs, a.heads, a.table_width, a.window);
   const uint32_t page_tiles = uint32_t(cache->page_size / hg::kTile);
-  hg::AttentionParams p{*cache, a, nullptr, nullptr, 0, 0, 0, 0.f, std::max(1, a.table_width / 32 + (a.table_width % 32 ? 1 : 0)), s.head_units, s.chunks, a.heads / cache->kv_heads, s.split, s.ring, page_tiles,
+  hg::AttentionParams p{*cache, a, nullptr, nullptr, 0, 0, 0, 0.f, std::max(1, std::min(a.table_width / 32 + (a.table_width % 32 ? 1 : 0), hg::kTableLines / a.seqs)), s.head_units, s.chunks, a.heads / cache->kv_heads, s.split, s.ring, page_tiles,
                         uint32_t(((uint64_t(1) << 32) + page_tiles - 1) / page_tiles)};
   if (s.line) {
     if (!a.workspace) throw std::runtime_error("hg_attention: a workspace is needed");

@@ -123,7 +123,8 @@ class PagedCache:
         sequence that sees nothing (length 0) gives zeros and minus infinity.  A length beyond the table is cut to it, and the
         positions of a page number outside the cache (-1, say, where a page was given up) are left out.  What the table holds
         behind a sequence's last page, and the cache behind its last position, has no influence, NaNs included.
-        How the work is spread over the device is chosen by the table's width, so a table far wider than its sequences costs a few us.
+        How the work is spread over the device is chosen by the table's width, so a table far wider than its sequences costs a few us
+        (one sequence of 1000 positions 5.2 us with 64 columns, 9.8 with 2048); `page_table[:, :n]` will do.
         """
         return self._attend(q, page_table, lengths, scale, window, lse, False)
 
