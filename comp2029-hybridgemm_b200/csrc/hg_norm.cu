@@ -18,8 +18,7 @@ namespace hg {
 namespace {
 
 constexpr int kNormThreads = 1024, kNormVectors = 4;   // at most kNormThreads x kNormVectors x 8 columns
-constexpr int kManyRows = 768;
-constexpr int kWideThreads = 448, kWideWork = 9 << 16, kThreadsPerSm = 1120;
+constexpr int kManyRows = 768, kWideRow = 3200, kMuch = 1 << 23;
 
 // Sum over the block; `parts` holds a float for each warp and is used once.
 __device__ __forceinline__ float block_sum(float v, float4* parts) {
@@ -138,65 +137,48 @@ __device__ __forceinline__ void pad_scales(const hg_norm_call& p, int first) {
     *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.scales) + scale_word_offset(p.rows + int(i / kblocks), int(i % kblocks), p.k)) = 0x7f7f7f7fu;
 }
 
-// A block to a row, eight columns to a thread and vector.  MANY: blocks go on to further rows, `row_blocks` behind, whose loads are under way
-// while the one before is summed and written.
-template <typename T, int VECTORS, bool MANY>
+// Few or wide rows: a block to a row, eight columns to a thread and vector.
+template <typename T, int VECTORS>
 __global__ void __launch_bounds__(kNormThreads)
-norm_kernel(const hg_norm_call p, const int row_blocks) {
-  __shared__ float4 parts[MANY ? 4 : 2][8];
+norm_kernel(const hg_norm_call p) {
+  __shared__ float4 parts[2][8];
   pdl_trigger();
-  if (blockIdx.x >= unsigned(row_blocks)) return pad_scales(p, row_blocks);
+  const int row = blockIdx.x;
+  if (row >= p.rows) return pad_scales(p, p.rows);
   pdl_wait();
   const float inv_k = 1.f / float(p.k);
-  uint4 x[VECTORS], weight[VECTORS], residual[VECTORS];
-  const auto fetch = [&](int row) {
-#pragma unroll
-    for (int j = 0; j < VECTORS; ++j) {
-      const int col = (j * blockDim.x + threadIdx.x) * 8;
-      if (col >= p.k) continue;
-      x[j] = *at(p.x, row * p.x_stride + col);
-      if (p.residual) residual[j] = *at(p.residual, row * p.residual_stride + col);
-    }
-  };
-#pragma unroll
-  for (int j = 0; j < VECTORS; ++j) x[j] = residual[j] = weight[j] = make_uint4(0, 0, 0, 0);
-  fetch(blockIdx.x);
+  uint4 h[VECTORS], weight[VECTORS], residual[VECTORS];
+  float sum = 0.f;
 #pragma unroll
   for (int j = 0; j < VECTORS; ++j) {
     const int col = (j * blockDim.x + threadIdx.x) * 8;
-    if (col < p.k) weight[j] = *at(p.weight, col);
+    h[j] = residual[j] = weight[j] = make_uint4(0, 0, 0, 0);
+    if (col >= p.k) continue;
+    h[j] = *at(p.x, row * p.x_stride + col);
+    if (p.residual) residual[j] = *at(p.residual, row * p.residual_stride + col);
+    weight[j] = *at(p.weight, col);
   }
-  int turn = 0;   // a row's sums are read while the next one's are written elsewhere
-  for (int row = blockIdx.x;;) {
-    float sum = 0.f, r = 1.f;
-    if (p.post_weight) {
+  float r = 1.f;
+  if (p.post_weight) {
 #pragma unroll
-      for (int j = 0; j < VECTORS; ++j) sum += squares8<T>(x[j]);
-      r = inverse_root(block_sum(sum, parts[2 * turn]) * inv_k + p.post_eps);
-    }
-    sum = 0.f;
-    uint4 h[VECTORS];
+    for (int j = 0; j < VECTORS; ++j) sum += squares8<T>(h[j]);
+    r = inverse_root(block_sum(sum, parts[0]) * inv_k + p.post_eps);
+  }
+  sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < VECTORS; ++j) {
-      const int col = (j * blockDim.x + threadIdx.x) * 8;
-      h[j] = x[j];
-      if (changes(p) && col < p.k) {
-        h[j] = stream8<T>(p, row, col, h[j], r, residual[j]);
-        *at(p.stream_out, int64_t(row) * p.k + col) = h[j];
-      }
-      sum += squares8<T>(h[j]);
+  for (int j = 0; j < VECTORS; ++j) {
+    const int col = (j * blockDim.x + threadIdx.x) * 8;
+    if (changes(p) && col < p.k) {
+      h[j] = stream8<T>(p, row, col, h[j], r, residual[j]);
+      *at(p.stream_out, int64_t(row) * p.k + col) = h[j];
     }
-    const int next = row + row_blocks;
-    if (MANY && next < p.rows) fetch(next);
-    r = inverse_root(block_sum(sum, parts[2 * turn + 1]) * inv_k + p.eps);
+    sum += squares8<T>(h[j]);
+  }
+  r = inverse_root(block_sum(sum, parts[1]) * inv_k + p.eps);
 #pragma unroll
-    for (int j = 0; j < VECTORS; ++j) {
-      const int col = (j * blockDim.x + threadIdx.x) * 8;
-      if (col < p.k) emit8<T>(p, row, col, h[j], weight[j], r);
-    }
-    if (!MANY || next >= p.rows) return;
-    row = next;
-    turn ^= 1;
+  for (int j = 0; j < VECTORS; ++j) {
+    const int col = (j * blockDim.x + threadIdx.x) * 8;
+    if (col < p.k) emit8<T>(p, row, col, h[j], weight[j], r);
   }
 }
 
@@ -207,16 +189,14 @@ void launch_norm(const hg_norm_call& p, cudaStream_t stream) {
   const int pad_words = p.codes ? (((p.rows + 127) & ~127) - p.rows) * (p.k >> 7) : 0;
   // One vector gives the shorter chain while SMs hold few rows (3584 columns: one row 1.8 us, with two 2.1; 512 rows 4.0 and 4.4), two halve
   // the barriers and weigh less on issue where they hold many (2048 rows 11.6 us and 10.5; 1024 rows of 2432 with a post norm and a gate 7.5
-  // and 6.6).  A warp to a row, without barriers, was slower everywhere (2048 rows 16.2 us): too few rows under way.
-  const int vectors = p.k <= kNormThreads * 8 && (p.rows < kManyRows || p.k <= 1024) ? 1 : p.k <= kNormThreads * 16 ? 2 : kNormVectors;
+  // and 6.6), and four leave an SM more rows at once where there are rows enough for that (16384 x 4096 85.7 us and 72.9, 2048 x 5120 15.7 and
+  // 14.4, 2048 x 12288 47.7 and 35.8; but 2048 x 3584 10.5 and 10.8, 4096 x 2432 13.9 and 14.2, 8192 x 1152 14.4 and 16.1).  A warp to a row,
+  // without barriers, was slower everywhere (2048 rows 16.2 us): too few rows under way.
+  const bool much = p.k >= kWideRow && int64_t(p.rows) * p.k >= kMuch;
+  const int vectors = much ? kNormVectors : p.k <= kNormThreads * 8 && (p.rows < kManyRows || p.k <= 1024) ? 1 : p.k <= kNormThreads * 16 ? 2 : kNormVectors;
   const int threads = ((p.k + 8 * vectors - 1) / (8 * vectors) + 31) & ~31, pad_blocks = std::min((pad_words + threads - 1) / threads, 16);
-  // Wide rows leave an SM two blocks or one, which wait for memory together: these go on from row to row, with the next row's loads under way (2048
-  // rows of 7168 columns 23.8 us and 20.8, of 8192 25.9 and 22.5, of 12288 47.7 and 34.7; 1024 of 8192 13.6 both, with a post norm and a gate 18.7 and
-  // 20.1).  Narrower rows have blocks enough (3584: 10.5 and 11.4).
-  const bool many = vectors == 2 && threads >= kWideThreads && int64_t(p.rows) * threads >= kWideWork;
-  const int row_blocks = many ? std::min(p.rows, sm_count() * std::max(1, kThreadsPerSm / threads)) : p.rows;
-  const auto kernel = many ? norm_kernel<T, 2, true> : vectors == 1 ? norm_kernel<T, 1, false> : vectors == 2 ? norm_kernel<T, 2, false> : norm_kernel<T, kNormVectors, false>;
-  check(launch_kernel(kernel, dim3(unsigned(row_blocks + pad_blocks)), dim3(threads), 0, stream, p, row_blocks), "norm");
+  const auto kernel = vectors == 1 ? norm_kernel<T, 1> : vectors == 2 ? norm_kernel<T, 2> : norm_kernel<T, kNormVectors>;
+  check(launch_kernel(kernel, dim3(unsigned(p.rows + pad_blocks)), dim3(threads), 0, stream, p), "norm");
 }
 
 }  // namespace
