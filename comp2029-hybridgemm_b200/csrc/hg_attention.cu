@@ -291,9 +291,10 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
   // Lengths and tables come as far as L2 while the kernel in front ends (from cold memory 4 x 32768 tokens took 31.8 us for 32.2 without);
   // what they hold is read behind the wait.
   {
-    const int at = int(blockIdx.x * kThreads + threadIdx.x), row = at / p.table_lines;
+    const unsigned at = blockIdx.x * kThreads + threadIdx.x, row = at / unsigned(p.table_lines), col = (at - row * p.table_lines) * 32;
     if (threadIdx.x * 32 < p.call.seqs) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.call.lengths + threadIdx.x * 32));
-    if (row < p.call.seqs) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.call.table + row * p.call.table_stride + (at - row * p.table_lines) * 32));
+    if (row < unsigned(p.call.seqs) && col < unsigned(p.call.table_width))
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.call.table + int64_t(row) * p.call.table_stride + col));
   }
   // Loads below are ordinary ones: the kernel in front may still be writing the cache when this one starts, so the data is not
   // read-only for its duration.
