@@ -83,6 +83,7 @@ def _norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, packed):
             raise ValueError("norm requires a gate with contiguous rows aligned to 16 bytes")
     if _differentiated(x, weight, residual, gate, post_weight):
         raise ValueError("norm has no gradient")
+    scale = C.c_float(scale).value   # as the kernel takes it: whether the stream changes is decided by the same number there
     changed = residual is not None or gate is not None or post_weight is not None or scale != 1.0
     stream = torch.empty((rows, k), dtype=x.dtype, device=x.device) if changed else x
     normed = codes = sf = None

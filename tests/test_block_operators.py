@@ -1,5 +1,6 @@
 """What stands between the linears, without a GPU: refusals of the C entries before any launch, of the Python calls for tensors that are not
 on a GPU, the registered op of a layer with an epilogue, and the way a vLLM layer's bias takes."""
+import contextlib
 import ctypes as C
 
 import pytest
@@ -129,6 +130,32 @@ def test_python_calls_refuse_what_is_not_on_a_gpu():
     for bad in (dict(pages=0), dict(kv_heads=0), dict(page_size=0)):
         with pytest.raises(ValueError):
             PagedCache.allocate(**(dict(pages=2, page_size=16, kv_heads=1, head_dim=64, device="cpu") | bad))
+
+
+class OnGpu(torch.Tensor):
+    """Stands in for a tensor on a GPU where no kernel runs."""
+    is_cuda = True
+
+
+@pytest.mark.parametrize("scale, changes", [(1.0, False), (1 + 1e-9, False), (2 ** .5 * .5 ** .5, False), (1 + 2.0 ** -22, True), (0.0, True)])
+def test_a_stream_is_returned_where_the_kernel_writes_one(scale, changes, monkeypatch):
+    """The kernel decides by the scale in fp32."""
+    calls = []
+
+    class Library:
+        @staticmethod
+        def hg_norm(call, dtype, stream):
+            calls.append(call._obj)
+            return 0
+
+    monkeypatch.setattr(native, "_host", None)
+    monkeypatch.setattr(producer, "library", lambda: Library)
+    monkeypatch.setattr(producer, "_on_device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(producer, "_stream", lambda device: 0)
+    x, weight = (torch.ones(shape, dtype=torch.bfloat16).as_subclass(OnGpu) for shape in ((2, 256), 256))
+    for call in (producer.norm, producer.norm_pack):
+        h = call(x, weight, scale=scale)[-1]
+        assert (h is not x) == changes == (calls[-1].scale != 1.0) and bool(calls[-1].stream_out) == changes
 
 
 class Layer:

@@ -214,3 +214,19 @@ def test_refusals(change, message):
             call(x, weight, 1e-6, **a)
     with pytest.raises(ValueError, match="gradient"):
         producer.norm(torch.zeros(2, 256, dtype=torch.bfloat16, device="cuda").requires_grad_(), torch.zeros(256, dtype=torch.bfloat16, device="cuda"))
+
+
+@pytest.mark.parametrize("way", ["extension", "ctypes"])
+def test_a_scale_that_rounds_to_one(way, monkeypatch):
+    """The kernel takes the scale in fp32: one that is 1 there leaves the stream as it is, whichever way the call goes."""
+    a = inputs(4, 256, torch.bfloat16, False, None, 1.0, False)
+    producer.norm(a["x"], a["weight"])
+    if way == "ctypes":
+        monkeypatch.setattr(native, "_host", None)
+    for scale in (1 + 1e-9, 2 ** .5 * .5 ** .5, 1 - 2.0 ** -26):
+        held = torch.full((4, 256), float("nan"), dtype=torch.bfloat16, device="cuda")
+        del held   # what an allocation finds there
+        assert producer.norm(a["x"], a["weight"], scale=scale)[1] is a["x"]
+        assert producer.norm_pack(a["x"], a["weight"], scale=scale)[2] is a["x"]
+    n, h = producer.norm(a["x"], a["weight"], scale=1 + 2.0 ** -22)   # not 1 in fp32, and nothing for bf16
+    assert h is not a["x"] and torch.equal(h, a["x"])
