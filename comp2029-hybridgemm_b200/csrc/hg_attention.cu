@@ -20,11 +20,13 @@
 // dependent loads and two meetings of blocks are all but 0.2.
 //
 // Roundings: q keeps its 16 bits (a head's bf16 queries become halves under a power of two, which keeps eight bits of all that is
-// not 2^-29 of the largest).  P times the scale of its values is rounded to 11 bits (2^-11 of each weight at most), held
-// between 2^-32 and 2^8 of the largest so far by a bias of 2^7 and lazy rescaling.  Sums, maxima and outputs are fp32.  Where the output
-// is quantised (EXACT) what the rounding of P left goes through a second product: an output beside the border of two scales changes the codes
-// of its whole group, and a rounding to 16 bits no longer hides the difference.  (37 sequences, codes against 64-bit arithmetic:
-// relative difference 0.015 with one product, none with two, 0.010 in fp32 arithmetic; 16.6 us and 17.0.)
+// not 2^-29 of the largest).  P times the scale of its values is rounded to 11 bits (2^-11 of it at most) where it is 2^-21 or more of the largest
+// weight times the largest scale of its head and group so far, and off by up to 2^-32 of these where it is less: a bias of 2^7, a power of two for
+// each group and lazy rescaling hold it in the range of a half.  Weights are exponentials by ex2.approx (two units of fp32).  Sums, maxima and outputs
+// are fp32.  Where the output is quantised (EXACT) what the rounding of P left goes through a second product: an output beside the border of two scales
+// changes the codes of its whole group, and a rounding to 16 bits no longer hides the difference.  (37 sequences, values of
+// the codes against 64-bit arithmetic, relative: 0.015 with one product; with two, in five draws, 4e-20 to 3e-5, fp32 arithmetic 8e-8 to 1e-2: single
+// codes beside a border, on either side.)
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -62,7 +64,8 @@ constexpr int kTableLines = 8192;    // lines of the table that are prefetched, 
 constexpr int kSmBytes = 228 << 10;  // shared memory of an SM
 constexpr float kBias = 7.f, kSlack = 4.f;   // P is kept in [0, 2^(kBias + 2 kSlack)]
 constexpr float kNone = -3e38f;      // maximum of nothing
-constexpr int kLeastScale = 24;      // values are summed under 2^-103 at least
+constexpr int kLeastScale = 24, kMostScale = 250;   // values are summed under 2^-103 at least and 2^123 at most (bytes of E8M0)
+constexpr uint32_t kZeros = 0x7f7f7f7fu;   // scale bytes of groups of zeros
 
 // How units come to blocks.  Few units (CLUSTER): a cluster of `split` blocks each, whose sums meet in shared memory.  Many (LINE):
 // the work is a line on which every unit (sequence and head unit, in this order) has its tiles behind what it costs
@@ -122,6 +125,17 @@ __device__ __forceinline__ uint32_t max_pairs(uint32_t a, uint32_t b) {
   const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&m);
 }
+__device__ __forceinline__ uint32_t min_pairs(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t mul_pairs(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+// 2^(byte - 127) twice, and the inverse of a pair of powers of two.
+__device__ __forceinline__ constexpr uint32_t pair_of(int byte) { return uint32_t(byte) * 0x00800080u; }
+__device__ __forceinline__ uint32_t inverse_pair(uint32_t a) { return pair_of(254) - a; }
 __device__ __forceinline__ float power_of(int biased) { return __uint_as_float(uint32_t(biased) << 23); }
 
 __device__ __forceinline__ uint4 shared_16(uint32_t at) {
@@ -198,7 +212,7 @@ __device__ __forceinline__ void write_out(const AttentionParams& p, int seq, int
   else
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.call.out) + (int64_t(seq) * p.call.heads + head) * kDim + d) =
         make_uint2(uint32_t(from_float<T>(v[0])) | (uint32_t(from_float<T>(v[1])) << 16), uint32_t(from_float<T>(v[2])) | (uint32_t(from_float<T>(v[3])) << 16));
-  if (p.call.lse && d == 0) p.call.lse[int64_t(seq) * p.call.heads + head] = l == 0.f ? -INFINITY : (m - kBias + log2f(l)) * 0.69314718f;
+  if (p.call.lse && d == 0) p.call.lse[int64_t(seq) * p.call.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718f;
 }
 
 // Adds the sums of `count` other blocks, in their order, to m, l and sum; `load(j, sums, {maximum, weight})` for some of them together.
@@ -503,10 +517,13 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) out[g][h][i] = 0.f;
-    // Heads 2c and 2c + 1.  Weights (of this lane's tokens) and values are summed over 2^(maximum + value_scale - 127 - kBias).
+    // Heads 2c and 2c + 1.  Weights (of this lane's tokens) are summed over 2^(maximum - kBias), values over that and the scale of their group.
     float maximum[2] = {kNone, kNone}, weight[2] = {0.f, 0.f};
     float2 shift = make_float2(-kNone, -kNone);
-    int value_scale = kLeastScale;
+    uint32_t inverse[GROUPS / 2];   // pairs of 1 / (the scale of a group's sums)
+#pragma unroll
+    for (int j = 0; j < GROUPS / 2; ++j) inverse[j] = pair_of(254 - kLeastScale);
+    const auto scale_byte = [&](int g) { return 254 - int((inverse[g / 2] >> (g & 1 ? 23 : 7)) & 255u); };
 
     for (int t = begin + warp; t < end; t += WARPS) {
       if (!lost && !warp_wait(bars + 8 * stage, phase, &given_up)) {
@@ -552,7 +569,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
 #pragma unroll
         for (int j = 0; j < GROUPS / 2; ++j) {
           key_scales[i][j] = two_scales(ks[i] >> (16 * j));
-          value_scales[i][j] = two_scales(vs[i] >> (16 * j));
+          value_scales[i][j] = mul_pairs(two_scales(vs[i] >> (16 * j)), inverse[j]);
         }
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
@@ -601,7 +618,6 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
           }
         }
       }
-      float scale[2][GROUPS];
       const float2 first = add2(sum[0], shift), second = add2(sum[1], shift);
       float x[4] = {first.x, first.y, second.x, second.y};
       if (!whole_tile) {
@@ -609,41 +625,75 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
         for (int i = 0; i < 4; ++i)
           if (!seen[i >> 1]) x[i] = -INFINITY;
       }
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) scale[i][g] = scale_of(value_scales[i][g / 2], g);
       uint32_t tops = max_pairs(value_scales[0][0], value_scales[1][0]);
       if constexpr (GROUPS == 4) tops = max_pairs(tops, max_pairs(value_scales[0][1], value_scales[1][1]));
-      const float top = fmaxf(scale_of(tops, 0), scale_of(tops, 1));
 
-      // A new maximum, or larger scales of the values, is taken up only when a weight could leave the range of a half.
-      const bool rescale = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > float(127 - value_scale) + (kBias + kSlack) || top > power_of(value_scale) * 16.f;
-      if (__any_sync(0xffffffffu, rescale)) {
-        const int new_scale = max(value_scale, min(254, int(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23)));
-        const float shrink = power_of(max(0, 127 + value_scale - new_scale));
-        value_scale = new_scale;
+      // A new maximum, or a larger scale of a group's values, is taken up only when a weight could leave the range of a half.
+      const bool larger = (tops + 0x3e003e00u) & 0x80008000u;   // more than 16 times
+      const bool higher = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > kBias + kSlack;
+      if (__any_sync(0xffffffffu, larger || higher)) {
+        // Groups of zeros have the scale 2^0, which says nothing of the others, so they do not count.  They are looked for where a byte could be theirs.
+        // A group that holds nothing else brings every tile here (128 x 1100 tokens with the last group of 128 empty 39.8 us for 32.2); to know that of it
+        // cost every tile 2 %.
+        if (__builtin_expect(__any_sync(0xffffffffu, __vcmpeq4(vs[0], kZeros) | __vcmpeq4(vs[1], kZeros)), 0)) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t codes[4] = {0, 0, 0, 0}, live = 0;   // of the groups, a quarter of them in a lane
+#pragma unroll
+            for (int j = 0; j < GROUPS / 2; ++j) {
+              const uint4 w = shared_16(values + (key_at ^ (64 * j)) + i * 8 * kDim);
+              codes[0] |= w.x; codes[1] |= w.y; codes[2 % GROUPS] |= w.z; codes[3 % GROUPS] |= w.w;
+            }
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) live |= codes[g] & 0x7f7f7f7fu ? 0xffu << (8 * g) : 0;
+            live |= __shfl_xor_sync(0xffffffffu, live, 1);
+            live |= __shfl_xor_sync(0xffffffffu, live, 2);
+            vs[i] &= live;
+          }
+        }
+        uint32_t shrink[GROUPS / 2];
+#pragma unroll
+        for (int j = 0; j < GROUPS / 2; ++j) {
+          value_scales[0][j] = two_scales(vs[0] >> (16 * j));
+          value_scales[1][j] = two_scales(vs[1] >> (16 * j));
+          uint32_t top = max_pairs(value_scales[0][j], value_scales[1][j]);
+#pragma unroll
+          for (int step = 4; step < 32; step <<= 1) top = max_pairs(top, __shfl_xor_sync(0xffffffffu, top, step));
+          top = min_pairs(top, pair_of(kMostScale));
+          const uint32_t before = inverse_pair(inverse[j]);
+          inverse[j] = inverse_pair(max_pairs(before, top));
+          shrink[j] = mul_pairs(before, inverse[j]);
+          value_scales[0][j] = mul_pairs(value_scales[0][j], inverse[j]);
+          value_scales[1][j] = mul_pairs(value_scales[1][j], inverse[j]);
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float m = fmaxf(seen[0] ? s[h] : kNone, seen[1] ? s[h + 2] : kNone);
 #pragma unroll
           for (int step = 4; step < 32; step <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, step));
           m = fmaxf(m, maximum[h]);
-          const float factor = exp2_fast(maximum[h] - m) * shrink;
+          const float factor = exp2_fast(maximum[h] - m);
           maximum[h] = m;
-          (h ? shift.y : shift.x) = float(127 - value_scale) + kBias - m;
+          (h ? shift.y : shift.x) = kBias - m;
           weight[h] *= factor;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            x[h + 2 * i] = seen[i] ? s[h + 2 * i] + (h ? shift.y : shift.x) : -INFINITY;
+          for (int i = 0; i < 2; ++i) x[h + 2 * i] = seen[i] ? s[h + 2 * i] + (h ? shift.y : shift.x) : -INFINITY;
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-              out[g][i][h] *= factor;
-              out[g][i][h + 2] *= factor;
+          for (int g = 0; g < GROUPS; ++g) {
+            const float by = factor * scale_of(shrink[g / 2], g);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              out[g][i][h] *= by;
+              out[g][i][h + 2] *= by;
             }
           }
         }
       }
+      float scale[2][GROUPS];
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) scale[i][g] = scale_of(value_scales[i][g / 2], g);
       float2 probability[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) probability[i] = make_float2(exp2_fast(x[2 * i]), exp2_fast(x[2 * i + 1]));
@@ -714,22 +764,24 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
 
     // The block's warps meet: sums under a common maximum.
     __syncthreads();   // the rings are idle, and sums that were there have been read
-    const float unit_scale = lost ? __uint_as_float(0x7fc00000u) : mx_scale(value_scale);
+    const float unit = lost ? __uint_as_float(0x7fc00000u) : power_of(127 - int(kBias));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int step = 4; step < 32; step <<= 1) weight[h] += __shfl_xor_sync(0xffffffffu, weight[h], step);
       if (r == 0) {
-        weights[warp][2 * c + h] = weight[h] * unit_scale;
+        weights[warp][2 * c + h] = weight[h] * unit;
         maxima[warp][2 * c + h] = maximum[h];
       }
     }
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g)
+    for (int g = 0; g < GROUPS; ++g) {
+      const float group = lost ? unit : power_of(scale_byte(g) - int(kBias));
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         *reinterpret_cast<float4*>(&sums[warp][2 * c + h][32 * g + 4 * r]) =
-            make_float4(out[g][0][h] * unit_scale, out[g][0][h + 2] * unit_scale, out[g][1][h] * unit_scale, out[g][1][h + 2] * unit_scale);
+            make_float4(out[g][0][h] * group, out[g][0][h + 2] * group, out[g][1][h] * group, out[g][1][h + 2] * group);
+    }
     __syncthreads();
     if constexpr (LINE && !kApart) find_others();
     if (others) {

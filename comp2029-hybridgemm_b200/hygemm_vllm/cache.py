@@ -123,6 +123,9 @@ class PagedCache:
         sequence that sees nothing (length 0) gives zeros and minus infinity.  A length beyond the table is cut to it, and the
         positions of a page number outside the cache (-1, say, where a page was given up) are left out.  What the table holds
         behind a sequence's last page, and the cache behind its last position, has no influence, NaNs included.
+        The weight of a position times the scale of 32 of its channels is rounded to 11 bits; where that is less than 2^-21 of the largest weight
+        times the largest scale that these channels have in the sequence, it is off by up to 2^-32 of the latter (`attention_pack` adds what the rounding
+        left).  Channels that hold only zeros change nothing of the others, but a head padded with 32 of them takes a quarter longer.
         How the work is spread over the device is chosen by the table's width, so a table far wider than its sequences costs a few us
         (one sequence of 1000 positions 5.2 us with 64 columns, 9.8 with 2048); `page_table[:, :n]` will do.
         """

@@ -247,6 +247,54 @@ def test_scores_and_scales_of_every_size(dtype):
         assert bool(got.isfinite().all())
 
 
+GROUPS_OF_VALUES = [
+    # types, exponent of each scale group's values, tokens (of 48) whose values are zeros, of which groups
+    (TYPES, [-13, -13, -13, None], "none", ()),                 # a head padded with zeros: 2^-13 is 1.2e-4
+    (TYPES, [None, -8, None, -13], "none", ()),
+    ([torch.bfloat16], [-20, -20, -20, None], "none", ()),
+    ([torch.bfloat16], [-80, None, -60, -40], "none", ()),
+    (TYPES, [10, -2, -8, -13], "none", ()),
+    ([torch.bfloat16], [30, 10, -10, -30], "none", ()),
+    ([torch.bfloat16], [0, -40, -80, 40], "none", ()),
+    ([torch.bfloat16], [100, -90, 60, 118], "none", ()),        # up to 2^120: sums stay in range
+    (TYPES, [-13, -13, -13, -13], "every third", (0, 1, 2, 3)),  # zeros between small values
+    ([torch.bfloat16], [-20, 0, -40, -20], "every third", (0, 1, 2)),
+    ([torch.bfloat16], [-20, -20, 0, -40], "the first", (0, 3)),  # zeros only, then small values
+    ([torch.bfloat16], [-20, -20, 8, -40], "the last", (0, 2, 3)),
+    ([torch.bfloat16], [-20, 0, -30, -40], "but one", (0, 2)),   # zeros only, up to one
+]
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim, lengths", [(8, 2, 128, [333, 1500, 17]), (4, 2, 64, [1500, 40]), (28, 4, 128, [300] * 64), (3, 1, 64, [700] * 160)])
+@pytest.mark.parametrize("case", range(len(GROUPS_OF_VALUES)))
+def test_values_of_groups_of_every_size(case, heads, kv_heads, dim, lengths):
+    """The scale groups of a head differ by any factor, or are zeros, in all entries or in some: each output is as near as its own group's values allow.
+    Sixteen bits add half a step; quantised outputs are held to fp32's error and the rounding of a weight alone."""
+    types, exponents, where, zero_groups = GROUPS_OF_VALUES[case]
+    for dtype in types:
+        cache, q, table, n = filled(len(lengths), heads, kv_heads, dim, 16, lengths, dtype, seed=case)
+        g = torch.Generator(device="cuda").manual_seed(case + 1)
+        position = torch.cat([torch.arange(m, device="cuda") for m in lengths])
+        slots = torch.cat([table[i].long()[torch.arange(m, device="cuda") // 16] * 16 + torch.arange(m, device="cuda") % 16 for i, m in enumerate(lengths)])
+        k, v = (torch.randn(slots.numel(), kv_heads, dim, device="cuda", generator=g) for _ in (0, 1))
+        zero = {"none": position < 0, "every third": position % 3 == 0, "the first": position < 210, "the last": position >= 20, "but one": position != 14}[where]
+        for group in range(dim // 32):
+            part = v[..., 32 * group:32 * group + 32]
+            part.mul_(0.0 if exponents[group] is None else 2.0 ** exponents[group])
+            if group in zero_groups:
+                part[zero] = 0
+        cache.write(k.to(dtype), v.to(dtype), slots)
+        got, lse = cache.attention(q, table, n, lse=True)
+        want, sums, size, score = reference(cache, q, table, n, dim ** -0.5)
+        assert bool(((got.double() - want).abs() <= bounds(dtype, want, size, score)).all())
+        assert bool(((lse.double() - sums).abs() <= 2.0 ** -17 * score + 2.0 ** -18 + 2.0 ** -22 * sums.abs()).all())
+        if heads * dim % 128 == 0:
+            codes, sf, packed_lse = cache.attention_pack(q, table, n, lse=True)
+            assert torch.equal(packed_lse, lse)
+            weight = 2.0 ** -11 + 2 * (2.0 ** -17 * score + 2.0 ** -18)
+            check_packed(codes, sf, want.flatten(1), (weight.unsqueeze(-1) * size).flatten(1))
+
+
 @pytest.mark.parametrize("amplitude", [0.0, 2.0 ** -100, 2.0 ** 60])
 def test_queries_of_every_size(amplitude):
     """bf16 queries beyond the range of a half: the scores are what they are, with a scale that brings them back."""
