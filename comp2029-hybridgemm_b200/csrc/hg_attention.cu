@@ -36,6 +36,7 @@
 
 #include "hg_cache.cuh"
 #include "hg_gemm_cluster.cuh"
+#include "hg_tags.cuh"
 
 namespace hg {
 namespace {
@@ -74,8 +75,8 @@ constexpr uint32_t kZeros = 0x7f7f7f7fu;   // scale bytes of groups of zeros
 // parts of it first, write their sums to a slot and set a tag behind them, and the first one waits for the tags and takes them back.
 // It waits for blocks behind it alone, whose first parts wait for nothing, so the wait ends even where the device holds fewer blocks
 // than there are: all but one of them end.  A tag is 64 bits that a workspace holds by accident once in 2^64 slots, so that
-// it needs no clearing before a launch.  Every call has its own one, which a later call does not take for its tag where a wait was
-// given up, and replays of a captured one find the tags taken back.
+// it needs no clearing before a launch.  Every call has its own one; replays of a captured one share it, and find it taken back, where a wait was
+// given up too (hg_tags.cuh).
 constexpr uint64_t kTag = 0x9d3f6ac1e57b2481ull;
 
 struct AttentionParams {
@@ -239,19 +240,29 @@ __device__ __forceinline__ void meet(int count, float& m, float& l, float4& sum,
   }
 }
 
-// Waits until the tag is set; what was written before it is then visible.  False when it is not within about two seconds.
-__device__ __forceinline__ bool wait_for(const uint64_t* at, uint64_t tag) {
-  const long long start = clock64();
-  for (uint32_t spin = 1;; ++spin) {
-    uint64_t now;
-    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(now) : "l"(at) : "memory");
-    if (now == tag) return true;
-    if ((spin & 63u) == 0) {
-      __nanosleep(100);
-      if (clock64() - start > kWaitLimitCycles) return false;
+struct TagWord {
+  uint64_t* at;
+  // Until the tag is set; what was written before it is then visible.  False when it is not within about two seconds.
+  __device__ __forceinline__ bool wait(uint64_t tag) const {
+    const long long start = clock64();
+    for (uint32_t spin = 1;; ++spin) {
+      uint64_t now;
+      asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(now) : "l"(at) : "memory");
+      if (now == tag) return true;
+      if ((spin & 63u) == 0) {
+        __nanosleep(100);
+        if (clock64() - start > kWaitLimitCycles) return false;
+      }
     }
   }
-}
+  // What was written before it is visible to whoever finds `to`.
+  __device__ __forceinline__ uint64_t exchange(uint64_t to) const {
+    uint64_t before;
+    asm volatile("fence.acq_rel.gpu;\n atom.relaxed.gpu.global.exch.b64 %0, [%1], %2;" : "=l"(before) : "l"(at), "l"(to) : "memory");
+    return before;
+  }
+  __device__ __forceinline__ void store(uint64_t to) const { asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(at), "l"(to) : "memory"); }
+};
 
 // Whether sums have a place of their own on a line, so that the next unit's first tiles and queries come in while one's are added up: where three
 // tiles to a warp are left beside them (4 x 32768 tokens 31.9 -> 30.3 us, 16 of 10 to 16000 22.6 -> 19.3, 37 of 1 to 4099 18.0 -> 17.4, 64 x 500 14.65 ->
@@ -473,6 +484,8 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     enter();
     fetch();
   }
+  [[maybe_unused]] TagWord own_tag{p.tags + blockIdx.x};
+  [[maybe_unused]] uint64_t tag_before = 0;   // looked at when the block ends: its way through memory is not waited for here
   for (;;) {
     if constexpr (!kApart) {
       enter();
@@ -785,8 +798,10 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     __syncthreads();
     if constexpr (LINE && !kApart) find_others();
     if (others) {
-      for (int i = threadIdx.x; i < others; i += kThreads)
-        if (!wait_for(p.tags + blockIdx.x + 1 + i, p.tag)) given_up = 1;
+      for (int i = threadIdx.x; i < others; i += kThreads) {
+        TagWord word{p.tags + blockIdx.x + 1 + i};
+        if (!take_tag(word, p.tag)) given_up = 1;
+      }
       __syncthreads();
     }
     for (int i = threadIdx.x; i < done_heads * kDim / 4; i += kThreads) {   // whole groups of eight lanes
@@ -830,9 +845,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
     if constexpr (LINE) {
       if (!begins) {
         __syncthreads();
-        if (threadIdx.x == 0) asm volatile("fence.acq_rel.gpu;\n st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p.tags + blockIdx.x), "l"(p.tag) : "memory");
-      } else if (others) {
-        for (int i = threadIdx.x; i < others; i += kThreads) p.tags[blockIdx.x + 1 + i] = 0;
+        if (threadIdx.x == 0) tag_before = leave_tag(own_tag, p.tag);
       }
       if constexpr (!kApart) advance();
       if (remaining <= 0) break;
@@ -864,6 +877,7 @@ attention_kernel(const __grid_constant__ AttentionParams p, const __grid_constan
       break;
     }
   }
+  if constexpr (LINE) settle_tag(own_tag, p.tag, tag_before);
   if (lost) {   // time for what is still on its way to shared memory
     const long long start = clock64();
     while (clock64() - start < 400000ll) __nanosleep(1000);
