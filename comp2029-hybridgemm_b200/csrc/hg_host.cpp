@@ -14,6 +14,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
@@ -177,8 +178,10 @@ struct Unlocked {
 // Operands of `DualLinear.linear`: null, or what an epilogue takes.
 struct Added { const at::Tensor *bias, *residual; int activation; };
 
-// A gradient would be asked of it: the calls have none, and Python says so.
-bool differentiated(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+// A gradient would be asked of it, or it carries a tangent of forward mode: the calls have neither, and Python says so.
+bool differentiated(const at::Tensor& t) {
+  return (c10::GradMode::is_enabled() && t.requires_grad()) || (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode());
+}
 bool sixteen_bits(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
 bool aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
 int dtype_of(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? HG_DTYPE_BF16 : HG_DTYPE_F16; }

@@ -23,6 +23,7 @@ import warnings
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 
 class Problem(C.Structure):
@@ -177,8 +178,10 @@ def _on_device(device):
 
 
 def _differentiated(*tensors) -> bool:
-    """Whether a gradient would be asked of one of them: the calls of this package are forward only."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a gradient would be asked of one of them, or one carries a tangent of forward mode: the calls of this package have neither."""
+    tensors = [t for t in tensors if t is not None]
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+            or forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors))
 
 
 def pack(x: torch.Tensor, fp4: bool = False):

@@ -5,6 +5,7 @@ import ctypes as C
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from hygemm_vllm import native, ops, producer
@@ -230,3 +231,26 @@ def test_a_vllm_layers_bias(handle, monkeypatch):
     assert torch.equal(method.apply(None, X, bias.double()), want.double()) and torch.equal(method.apply(None, X, strided), want) and not calls
     monkeypatch.setattr(Layer, "takes_epilogue", lambda self: False)
     assert torch.equal(method.apply(None, X, bias), want) and not calls
+
+
+def test_what_asks_for_a_gradient():
+    """Recorded gradients and tangents of forward mode; neither where it is off."""
+    x, tangent = torch.randn(2, 4), torch.ones(2, 4)
+    assert not native._differentiated(x, None) and not native._differentiated()
+    leaf = x.clone().requires_grad_()
+    assert native._differentiated(None, leaf)
+    with torch.no_grad():
+        assert not native._differentiated(leaf)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, tangent)
+        assert native._differentiated(x, dual) and not native._differentiated(x)
+        with torch.no_grad():
+            assert native._differentiated(dual)      # turns recording off, tangents not
+        with torch.inference_mode():
+            assert not native._differentiated(dual)
+        with forward_ad._set_fwd_grad_enabled(False):
+            assert not native._differentiated(dual)
+    assert not native._differentiated(dual)
+    seen = []
+    torch.func.jvp(lambda t: seen.append(native._differentiated(t)) or t.sum(), (x,), (tangent,))
+    assert seen == [True]

@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from hygemm_vllm import native, producer
 from hygemm_vllm.cache import PagedCache, page_bytes
@@ -196,4 +197,34 @@ def test_no_gradient_is_asked_where_none_is_recorded():
                 got = calls()
             assert not got.requires_grad
     assert torch.equal(got, layer.linear(x, bias.detach()))
+    layer.close()
+
+
+@pytest.mark.parametrize("way", ["extension", "ctypes"])
+def test_tangents_of_forward_mode_are_refused(way, monkeypatch):
+    """The calls have no derivative: they say so for a tangent as for a recorded gradient, and take the tensor where forward mode is off."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, weight = torch.randn(3, 896, device="cuda", generator=g).bfloat16(), torch.randn(896, device="cuda", generator=g).bfloat16()
+    layer = native.DualLinear(torch.randn(640, 896, device="cuda", generator=g).bfloat16(), torch.arange(0, 640, 9, device="cuda"))
+    bias, residual = torch.randn(640, device="cuda", generator=g).bfloat16(), torch.randn(3, 640, device="cuda", generator=g).bfloat16()
+    cache, q, table, n = filled(3, 8, 2, 64, 16, [20, 3, 40], torch.bfloat16)
+    kv, slots = q[:, :2].contiguous(), torch.tensor([1, 2, -1], device="cuda")
+    layer.linear(x, bias)
+    if way == "ctypes":
+        monkeypatch.setattr(native, "_host", None)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [lambda f=f, args=args: f(*args) for f, args in [
+            (producer.norm, (dual(x), weight)), (producer.norm_pack, (x, dual(weight))), (producer.norm, (x, weight, 1e-6, dual(x))),
+            (cache.attention, (dual(q), table, n)), (cache.attention_pack, (dual(q), table, n)), (cache.write, (dual(kv), kv, slots)),
+            (cache.write, (kv, dual(kv), slots)), (layer.linear, (dual(x), bias)), (layer.linear, (x, dual(bias))),
+            (layer.linear, (x, bias, "relu", dual(residual)))]]
+        for call in calls:
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+            with forward_ad._set_fwd_grad_enabled(False):
+                call()
+            with torch.inference_mode():
+                call()
+        assert torch.equal(layer.linear(x, bias), layer.linear(x, bias.clone()))
     layer.close()
