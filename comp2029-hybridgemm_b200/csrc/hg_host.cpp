@@ -183,7 +183,9 @@ bool differentiated(const at::Tensor& t) {
   return (c10::GradMode::is_enabled() && t.requires_grad()) || (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode());
 }
 bool sixteen_bits(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
-bool aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+// A tensor without memory (under tracing, say) would be taken for an operand that is not there.
+bool held(const at::Tensor& t) { return t.const_data_ptr() || !t.numel(); }
+bool aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 && held(t); }
 int dtype_of(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? HG_DTYPE_BF16 : HG_DTYPE_F16; }
 
 PyObject* forward_checked(PyObject* self, const at::Tensor& x, long math, const Added* added = nullptr) {
@@ -210,13 +212,13 @@ PyObject* forward_checked(PyObject* self, const at::Tensor& x, long math, const 
     const auto type = r->output.dtype().toScalarType();
     if (r->explicit_schedule || differentiated(x)) Py_RETURN_NONE;
     if (const at::Tensor* bias = added->bias) {
-      if (bias->device() != r->device || bias->scalar_type() != type || bias->dim() != 1 || bias->size(0) != r->outputs || !bias->is_contiguous() || differentiated(*bias))
+      if (bias->device() != r->device || bias->scalar_type() != type || bias->dim() != 1 || bias->size(0) != r->outputs || !bias->is_contiguous() || !held(*bias) || differentiated(*bias))
         Py_RETURN_NONE;
       epilogue.bias = bias->const_data_ptr();
     }
     if (const at::Tensor* residual = added->residual) {
       if (residual->device() != r->device || residual->scalar_type() != type || residual->dim() != 2 || residual->size(0) != r->tokens ||
-          residual->size(1) != r->outputs || residual->stride(1) != 1 || differentiated(*residual))
+          residual->size(1) != r->outputs || residual->stride(1) != 1 || !held(*residual) || differentiated(*residual))
         Py_RETURN_NONE;
       epilogue.residual = residual->const_data_ptr();
       epilogue.residual_stride = residual->stride(0);
@@ -398,14 +400,14 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // A cache as the library takes it; false: `data` is not one.
 bool cache_of(const at::Tensor& data, long page_size, long head_dim, hg_cache* cache) {
-  if (!data.is_cuda() || data.scalar_type() != at::kByte || data.dim() != 3 || !data.is_contiguous() || data.size(0) > 0x7fffffff || data.size(1) > 0x7fffffff ||
+  if (!data.is_cuda() || data.scalar_type() != at::kByte || data.dim() != 3 || !data.is_contiguous() || !held(data) || data.size(0) > 0x7fffffff || data.size(1) > 0x7fffffff ||
       page_size <= 0 || page_size > 1024 || (head_dim != 64 && head_dim != 128) || data.size(2) != page_size * (2 * head_dim + head_dim / 16))
     return false;
   *cache = hg_cache{data.data_ptr(), int(data.size(0)), int(data.size(1)), int(page_size), int(head_dim)};
   return true;
 }
 bool slots_of(const at::Tensor& slots, const at::Tensor& data) {
-  return slots.device() == data.device() && slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() && slots.size(0) > 0 && slots.size(0) <= 0x7fffffff;
+  return slots.device() == data.device() && slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() && held(slots) && slots.size(0) > 0 && slots.size(0) <= 0x7fffffff;
 }
 
 // cache_write(data, page_size, head_dim, k, v, slots): True when done
@@ -424,7 +426,7 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
       const at::Tensor& t = i ? v : k;
       if (t.device() != data.device() || !sixteen_bits(t) || t.scalar_type() != k.scalar_type() || t.dim() != 3 || t.size(0) != slots.size(0) ||
           t.size(1) != cache.kv_heads || t.size(2) != head_dim || t.stride(2) != 1 || t.stride(0) % 4 || t.stride(1) % 4 ||
-          reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 8 || differentiated(t))
+          reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 8 || !held(t) || differentiated(t))
         Py_RETURN_NONE;
       strides[2 * i] = t.stride(0);
       strides[2 * i + 1] = t.stride(1);
@@ -487,7 +489,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       Py_RETURN_NONE;
     const int64_t seqs = q.size(0), heads = q.size(1);
     if (table.device() != data.device() || table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != seqs || (table.size(1) > 1 && table.stride(1) != 1) ||
-        lengths.device() != data.device() || lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != seqs || !lengths.is_contiguous())
+        lengths.device() != data.device() || lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != seqs || !lengths.is_contiguous() || !held(table) || !held(lengths))
       Py_RETURN_NONE;
     const int64_t positions = table.size(1) * page_size;
     if (positions > (1 << 30) || window < 0) Py_RETURN_NONE;

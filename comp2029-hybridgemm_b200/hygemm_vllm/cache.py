@@ -20,7 +20,7 @@ import ctypes as C
 import torch
 
 from . import native
-from .native import DTYPES, _differentiated, _on_device, _stream, check, library, scale_size
+from .native import DTYPES, _differentiated, _held, _on_device, _stream, check, library, scale_size
 
 
 class Cache(C.Structure):
@@ -86,6 +86,8 @@ class PagedCache:
             if x.numel() and (x.stride(2) != 1 or x.data_ptr() % 8 or x.stride(0) % 4 or x.stride(1) % 4):
                 raise ValueError("PagedCache.write requires contiguous heads aligned to 8 bytes")
         self._slots(slots)
+        if not _held(self.data, k, v, slots):
+            raise ValueError("PagedCache.write requires operands in memory")
         if _differentiated(k, v):
             raise ValueError("PagedCache.write has no gradient")
         if not shape[0]:
@@ -104,6 +106,8 @@ class PagedCache:
         self._slots(slots)
         if dtype not in DTYPES:
             raise ValueError("PagedCache.read gives FP16 or BF16")
+        if not _held(self.data, slots):
+            raise ValueError("PagedCache.read requires operands in memory")
         tokens = slots.shape[0]
         k, v = (torch.empty((tokens, self.kv_heads, self.head_dim), dtype=dtype, device=self.data.device) for _ in (0, 1))
         if tokens:
@@ -151,6 +155,8 @@ class PagedCache:
         seqs, heads, _ = q.shape
         if seqs and (q.stride(2) != 1 or (heads > 1 and q.stride(1) != self.head_dim) or (seqs > 1 and q.stride(0) % 8) or q.data_ptr() % 16):
             raise ValueError("PagedCache.attention requires contiguous query rows aligned to 16 bytes")
+        if not _held(self.data, q, page_table, lengths):
+            raise ValueError("PagedCache.attention requires operands in memory")
         if _differentiated(q):
             raise ValueError("PagedCache.attention has no gradient")
         if not (page_table.device == device and page_table.dtype == torch.int32 and page_table.ndim == 2 and page_table.shape[0] == seqs

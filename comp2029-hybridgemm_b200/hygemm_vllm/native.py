@@ -177,6 +177,11 @@ def _on_device(device):
     return _HERE if torch._C._cuda_getDevice() == device.index else _switched(device)
 
 
+def _held(*tensors) -> bool:
+    """Whether all of them have memory: one without (under tracing, say) would be taken for an operand that is not there."""
+    return all(t is None or not t.numel() or t.data_ptr() for t in tensors)
+
+
 def _differentiated(*tensors) -> bool:
     """Whether a gradient would be asked of one of them, or one carries a tangent of forward mode: the calls of this package have neither."""
     tensors = [t for t in tensors if t is not None]
@@ -338,6 +343,8 @@ class DualLinear:
         if residual is not None and not (residual.device == x.device and residual.dtype == self.dtype
                                          and residual.shape == (tokens, self.outputs) and (residual.stride(1) == 1 or self.outputs == 1)):
             raise ValueError("HyGEMM epilogue requires a residual [tokens, outputs] of the layer's type and device with contiguous rows")
+        if not _held(x, bias, residual):
+            raise ValueError("HyGEMM epilogue requires operands in memory")
         if _differentiated(x, bias, residual):
             raise ValueError("HyGEMM layers have no gradient")
         return Epilogue(None if bias is None else bias.data_ptr(), None if residual is None or not tokens else residual.data_ptr(),

@@ -14,7 +14,7 @@ import os
 import torch
 
 from . import native
-from .native import DTYPES, _differentiated, _on_device, _stream, check, library, scale_size
+from .native import DTYPES, _differentiated, _held, _on_device, _stream, check, library, scale_size
 from .ops import _runtimes, linear_silu  # noqa: F401  (re-exported, reference layout)
 
 MAX_FUSED_TOKENS = 128
@@ -81,6 +81,8 @@ def _norm(x, weight, eps, residual, gate, scale, post_weight, post_eps, packed):
         per_row = int(gate.ndim == 2 and gate.shape[1] == 1 and k != 1)
         if not per_row and (gate.stride(-1) != 1 or (rows > 1 and gate_stride % 8) or gate.data_ptr() % 16):
             raise ValueError("norm requires a gate with contiguous rows aligned to 16 bytes")
+    if not _held(x, weight, residual, gate, post_weight):
+        raise ValueError("norm requires operands in memory")
     if _differentiated(x, weight, residual, gate, post_weight):
         raise ValueError("norm has no gradient")
     scale = C.c_float(scale).value   # as the kernel takes it: whether the stream changes is decided by the same number there

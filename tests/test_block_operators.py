@@ -5,6 +5,7 @@ import ctypes as C
 
 import pytest
 import torch
+from torch._subclasses import FakeTensorMode
 from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
@@ -254,3 +255,29 @@ def test_what_asks_for_a_gradient():
     seen = []
     torch.func.jvp(lambda t: seen.append(native._differentiated(t)) or t.sum(), (x,), (tangent,))
     assert seen == [True]
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
+def test_tensors_without_memory_are_refused():
+    """As tracing has them: their address is zero, which would stand for an operand that is not there."""
+    with FakeTensorMode():
+        x, weight = torch.empty(2, 256, dtype=torch.bfloat16, device="cuda"), torch.empty(256, dtype=torch.bfloat16, device="cuda")
+        held = PagedCache(torch.empty(4, 2, page_bytes(16, 64), dtype=torch.uint8, device="cuda"), 16, 64)
+        kv, slots = torch.empty(2, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.empty(2, dtype=torch.int64, device="cuda")
+        table, lengths = torch.empty(2, 3, dtype=torch.int32, device="cuda"), torch.empty(2, dtype=torch.int32, device="cuda")
+    for call in (lambda: producer.norm(x, weight), lambda: producer.norm_pack(x, weight, residual=x), lambda: held.write(kv, kv, slots),
+                 lambda: held.read(slots), lambda: held.attention(kv, table, lengths), lambda: held.attention_pack(kv, table, lengths)):
+        with pytest.raises(ValueError, match="in memory"):
+            call()
+
+
+@pytest.mark.parametrize("missing", ["residual", "gate", "post_weight", "weight"])
+def test_an_operand_without_memory_is_not_left_out(missing):
+    class Nowhere(OnGpu):
+        def data_ptr(self):
+            return 0
+
+    operands = {name: torch.ones(shape, dtype=torch.bfloat16).as_subclass(Nowhere if name == missing else OnGpu)
+                for name, shape in (("x", (2, 256)), ("weight", 256), ("residual", (2, 256)), ("gate", 256), ("post_weight", 256))}
+    with pytest.raises(ValueError, match="in memory"):
+        producer._norm(operands["x"], operands["weight"], 1e-6, operands["residual"], operands["gate"], 1.0, operands["post_weight"], None, True)
