@@ -222,3 +222,21 @@ def test_a_decode_step(dtype):
         assert all(torch.equal(a, b) for a, b in zip(held, (h, y, a8, a_sf, h1, n8, n_sf, z, out, d8, d_sf)))
     for module in (qkv, o_proj, gate_up, down):
         module.close()
+
+
+@pytest.mark.parametrize("activation, relative", [("silu", 2.0 ** -19), ("gelu", 2.0 ** -17), ("gelu_tanh", 2.0 ** -16)])
+def test_small_results_of_activations(activation, relative):
+    """Every bf16 value from -8 to -2^-10, where a result is up to 2^-47 of its argument: within the rounding of the exponent (an argument of up to 71
+    of exp2, half a unit of fp32 in each of the steps to it), then rounded once.  Rounding keeps the order, so the bounds are rounded like the result."""
+    v = torch.arange(0x3A80, 0x4101, device="cuda").to(torch.int16).view(torch.bfloat16).neg()
+    v = torch.cat([v, v.new_zeros(-v.numel() % 128)])
+    assert v.min() == -8 and v[0] == -2.0 ** -10
+    layer = native.DualLinear(torch.zeros(v.numel(), 128, dtype=torch.bfloat16, device="cuda"), torch.arange(0, v.numel(), 5, device="cuda"))
+    x = v.double()
+    want = {"silu": x * torch.sigmoid(x), "gelu": 0.5 * x * torch.special.erfc(-x / math.sqrt(2)),
+            "gelu_tanh": x * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (x + 0.044715 * x ** 3))}[activation]
+    low, high = (want * (1 + relative)).bfloat16(), (want * (1 - relative)).bfloat16()
+    for tokens in (3, 40):   # quantised in the launch, and ahead of it
+        y = layer.linear(torch.ones(tokens, 128, dtype=torch.bfloat16, device="cuda"), v, activation)
+        assert bool(((low <= y) & (y <= high)).all())
+    layer.close()
