@@ -14,10 +14,11 @@
 // those of the keys multiply a group's partial sum, those of the values the probabilities, once for every group, before these are
 // rounded to halves.
 //
-// What bounds it: bytes of the cache, and nearly as soon a warp's way through a tile (about 435 instructions for 4224 bytes, issued in half
+// What bounds it: bytes of the cache, and nearly as soon a warp's way through a tile (about 445 instructions for 4224 bytes, issued in half
 // of the slots, with the ALU pipe busy as long; from L2 an SM keeps up with some 24 bytes a clock, and memory delivers 23.6).  28 heads on 4 of 128, bf16: 128 sequences of 1024 to 1150 tokens
-// 31.7 us (0.72 of the measured copy rate), 128 x 4000 about 94 us (0.88), 4 x 32768 30.3 us (0.70); 1 x 1000 5.2 us, of which launch, three
-// dependent loads and two meetings of blocks are all but 0.2.
+// 32.6 us (0.70 of the measured copy rate), 128 x 4000 about 94 us (0.89), 4 x 32768 30.6 us (0.69); 1 x 1000 5.4 us, of which launch, three
+// dependent loads and two meetings of blocks are all but 0.2.  (Where two sides are compared below, both are from before values were summed under a
+// scale for each group, which adds 1 to 3 % to either.)
 //
 // Roundings: q keeps its 16 bits (a head's bf16 queries become halves under a power of two, which keeps eight bits of all that is
 // not 2^-29 of the largest).  P times the scale of its values is rounded to 11 bits (2^-11 of it at most) where it is 2^-21 or more of the largest
